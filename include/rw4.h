@@ -444,6 +444,51 @@ int rw4_ring_stage(rw4_ring* ring, int32_t slot, size_t offset, const void* src,
 int rw4_ring_submit(rw4_ring* ring, int32_t slot, void* dst, size_t n, void* done_event);
 int rw4_ring_wait_compute(rw4_ring* ring, void* stream);
 
+/* ---- 8-bit weights and activations (W8A8) ---------------------------------------------------
+ * Rows of signed 8-bit codes with one fp32 scale a row: value = code * scale.  Activations are
+ * quantized per token (row) as they are produced, weights once per output channel (row).  The
+ * reference expands such checkpoints to a bf16 scratch copy on every fetch
+ * (CompressedTensorsBackend, rocketllm/quant/safetensors_quant.py:244-293); here the codes are
+ * multiplied as they are.
+ *
+ * Quantizing a row y:  a = max |y|, scale = a / 127, code = rint(y * (127 / a)), ties to even, in
+ * fp32.  A row with a < 2^-119 is stored as scale 0, codes 0; a row that holds a NaN or an
+ * infinity as scale NaN, codes 0 (what reads it is NaN).  `dtype` (RW4_F32, RW4_BF16, RW4_F16) is
+ * the type of every floating input; row strides are in elements, any value of at least 0 (rows
+ * may overlap); codes, hidden and out are contiguous.  1 <= K <= 131072; M = 0 does nothing.  Rows
+ * of 16-byte aligned addresses and strides with K a multiple of 8 take vector loads, any others
+ * scalar ones.
+ */
+
+/* codes, scale = quantized rows of x[M, K], or of silu(gate) * x when gate is not null
+ * (silu(g) = g / (1 + exp(-g)); the product of transformers' LlamaMLP before down_proj). */
+int rw4_int8_quantize(const void* x, int64_t x_stride, const void* gate, int64_t gate_stride,
+                      int32_t dtype, int64_t M, int64_t K, int8_t* codes, float* scale,
+                      void* stream);
+
+/* out[M, K] = codes * scale, rounded to out_dtype. */
+int rw4_int8_dequantize(const int8_t* codes, const float* scale, int64_t M, int64_t K, void* out,
+                        int32_t out_dtype, void* stream);
+
+/* hidden = x + residual rounded to dtype (residual and hidden both null: hidden is x itself), and
+ * codes, scale = quantized rows of hidden * rsqrt(mean(hidden^2) + eps) * weight, all in fp32.
+ * hidden may be residual or x itself (same address, contiguous rows). */
+int rw4_int8_rmsnorm(const void* x, int64_t x_stride, const void* residual,
+                     int64_t residual_stride, const void* weight, int32_t dtype, int64_t M,
+                     int64_t K, float eps, void* hidden, int8_t* codes, float* scale,
+                     void* stream);
+
+/* out[M, N] = scale[m] * weight_scale[n] * sum_k codes[m, k] weight[n, k] + bias[n]
+ * + residual[m, n], rounded once to out_dtype (the type of bias and residual, either of which may
+ * be null).  The integer sum is exact: K a multiple of 16, 16 <= K <= 131056.  codes and weight
+ * 16-byte aligned and contiguous; residual may be out itself.  M = 0 or N = 0 does nothing.
+ * path: 0 the library's choice, 1 the one-CTA tiles with K split over clusters, 2 the CTA-pair
+ * tiles; every path gives the same bits. */
+int rw4_int8_linear(const int8_t* codes, const float* scale, int64_t M, int64_t K,
+                    const int8_t* weight, const float* weight_scale, int64_t N, const void* bias,
+                    const void* residual, void* out, int32_t out_dtype, int32_t path,
+                    void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -137,6 +137,16 @@ SIGNATURES = {
     "rw4_xfer_stats": (ctypes.c_int, [_c_void_p, ctypes.POINTER(ctypes.c_uint64),
                                       ctypes.POINTER(ctypes.c_uint64),
                                       ctypes.POINTER(ctypes.c_uint64), ctypes.POINTER(_i32)]),
+    "rw4_int8_quantize": (ctypes.c_int, [_c_void_p, _i64, _c_void_p, _i64, _i32, _i64, _i64,
+                                         _c_void_p, _c_void_p, _c_void_p]),
+    "rw4_int8_dequantize": (ctypes.c_int, [_c_void_p, _c_void_p, _i64, _i64, _c_void_p, _i32,
+                                           _c_void_p]),
+    "rw4_int8_rmsnorm": (ctypes.c_int, [_c_void_p, _i64, _c_void_p, _i64, _c_void_p, _i32, _i64,
+                                        _i64, ctypes.c_float, _c_void_p, _c_void_p, _c_void_p,
+                                        _c_void_p]),
+    "rw4_int8_linear": (ctypes.c_int, [_c_void_p, _c_void_p, _i64, _i64, _c_void_p, _c_void_p,
+                                       _i64, _c_void_p, _c_void_p, _c_void_p, _i32, _i32,
+                                       _c_void_p]),
 }
 
 _lib = None

@@ -1,0 +1,688 @@
+// 8-bit matrix product of the W8A8 path on the 5th-generation tensor cores (sm_100a):
+//
+//   out[m, n] = round(scale[m] * weight_scale[n] * sum_k codes[m, k] * weight[n, k]
+//                     + bias[n] + residual[m, n])
+//
+// codes and weight are signed 8-bit rows (K innermost).  The sum is exact: tcgen05.mma kind::i8
+// accumulates in 32-bit integers in TMEM, and K <= 131056 keeps any sum of products of 8-bit codes
+// (at most 2^14 each) inside them.  So the result does not depend on tiles or splits; scales, bias
+// and residual are applied to it in fp32 and rounded once to the output's type.
+//
+// Both kernels put the weight rows on the M side of the MMA (the accumulator's 128 TMEM lanes) and
+// tokens on its N side (its columns): one token is then one column, and a call of any number of
+// tokens from one on reads no more weight bytes than there are.  Operand tiles are 128 bytes of K
+// wide (one 128-byte swizzle atom: four MMAs of K = 32), loaded by TMA through an mbarrier ring; the
+// ends of K, of the weight rows and of the tokens are zero-filled by TMA and never stored.
+//
+//   split kernel   one CTA for 128 weight rows x BN tokens (BN = 16 .. 256), K split over the CTAs
+//                  of a cluster when there are fewer tiles than SMs; the integer partial sums meet
+//                  in distributed shared memory (no workspace, no atomics).
+//   pair kernel    two CTAs (cta_group::2) share one 256 x 256 tile: each holds 128 weight rows and
+//                  half of the tokens' operand, so a byte of shared memory feeds twice the MMAs.
+//                  Persistent over tiles; the accumulator is double-buffered in TMEM so that the
+//                  epilogue of one tile runs under the MMAs of the next.
+//
+// Every TMA load is a plain per-CTA load.  Every mbarrier wait is bounded (rw4_tma.cuh).
+#include <cooperative_groups.h>
+
+#include <atomic>
+#include <cstdlib>
+
+#include "rw4_tcgen05.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace {
+
+using namespace rw4;
+
+constexpr int BK = 128;                  // bytes (= codes) of K per stage
+constexpr int BMW = 128;                 // weight rows per CTA
+constexpr int kWBytes = BMW * BK;        // 16 KB
+constexpr int64_t kMaxK = 131056;
+
+// Instruction descriptor, kind::i8: D s32 (2 << 4), A and B signed 8-bit (1 << 7, 1 << 10), both
+// K-major, N >> 3 at bit 17, M >> 4 at bit 24.
+__host__ __device__ constexpr uint32_t idesc_i8(int m, int n) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) |
+         ((uint32_t)(m >> 4) << 24);
+}
+
+struct Epilogue {
+  const float* scale;         // [M]
+  const float* weight_scale;  // [N]
+  const void* bias;           // [N] or null
+  const void* residual;       // [M, N] or null
+  void* out;                  // [M, N]
+};
+
+template <typename T>
+__device__ __forceinline__ float ep_f(T v);
+template <>
+__device__ __forceinline__ float ep_f(float v) { return v; }
+template <>
+__device__ __forceinline__ float ep_f(__half v) { return __half2float(v); }
+template <>
+__device__ __forceinline__ float ep_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T ep_t(float v);
+template <>
+__device__ __forceinline__ float ep_t(float v) { return v; }
+template <>
+__device__ __forceinline__ __half ep_t(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 ep_t(float v) { return __float2bfloat16_rn(v); }
+
+__device__ __forceinline__ void umma_i8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                        uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// 16 columns of this warp's 32 lanes, and 32 (tmem_ld32)
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+      "%12, %13, %14, %15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
+        "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
+        "=r"(v[14]), "=r"(v[15])
+      : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void pdl_wait() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+__device__ __forceinline__ void pdl_launch() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+// One weight row's share of the epilogue: `count` tokens from m on, sums in v (already in fp32
+// registers' integer form).  Adjacent lanes hold adjacent outputs n, so a warp's store of one token
+// is one run of 32 outputs.
+template <typename T, int COLS>
+__device__ __forceinline__ void store_cols(const Epilogue& e, const uint32_t (&v)[COLS], int m,
+                                           int M, int n, int N, float ws, float bias, float sx) {
+  const T* res = static_cast<const T*>(e.residual);
+  T* out = static_cast<T*>(e.out) + (int64_t)m * N + n;
+  const bool row = n < N;
+  T r[COLS];
+  if (res) {
+    res += (int64_t)m * N + n;
+#pragma unroll
+    for (int j = 0; j < COLS; ++j) r[j] = row && m + j < M ? res[(int64_t)j * N] : ep_t<T>(0.f);
+  }
+#pragma unroll
+  for (int j = 0; j < COLS; ++j) {
+    const float s = __shfl_sync(0xffffffffu, sx, j) * ws;
+    float y = fmaf(static_cast<float>(static_cast<int>(v[j])), s, bias);
+    if (res) y += ep_f(r[j]);
+    if (row && m + j < M) out[(int64_t)j * N] = ep_t<T>(y);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// split kernel
+// ---------------------------------------------------------------------------------------------
+
+template <int BN>
+struct SplitCfg {
+  static constexpr int kXBytes = BN * BK;
+  static constexpr int kStageBytes = kWBytes + kXBytes;
+  // up to 64 tokens two CTAs share an SM (one's prologue and epilogue under the other's loads)
+  static constexpr int kStages = BN == 16 ? 6 : BN == 32 ? 5 : BN == 64 ? 4 : BN == 128 ? 6 : 4;
+  static constexpr int kCtasPerSm = BN <= 64 ? 2 : 1;
+  static constexpr int kOffBars = kStages * kStageBytes;  // full[], empty[], accum
+  static constexpr int kOffTmem = kOffBars + (2 * kStages + 1) * 8;
+  static constexpr int kSmem = kOffTmem + 8 + 1024;
+  static constexpr uint32_t kTmemCols = BN < 32 ? 32 : BN;
+  static_assert(BN * BMW * 4 <= kStages * kStageBytes, "partial sums reuse the stages");
+  static_assert(kSmem * kCtasPerSm <= 227 * 1024 - 1024, "shared memory budget");
+};
+
+constexpr int kSplitThreads = 192;  // TMA, MMA, 4 epilogue warps
+
+template <int BN, typename T>
+__global__ void __launch_bounds__(kSplitThreads)
+    int8_split_kernel(const __grid_constant__ CUtensorMap tm_w,
+                      const __grid_constant__ CUtensorMap tm_x, const Epilogue e, int M, int N,
+                      int nkb, int m_tiles, unsigned int* status) {
+  using C = SplitCfg<BN>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~uintptr_t(1023));
+  __shared__ int aborted;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int splits = static_cast<int>(cluster.num_blocks());
+  const int rank = static_cast<int>(cluster.block_rank());
+  const int tile = blockIdx.x / splits;
+  const int m0 = (tile % m_tiles) * BN;   // tokens fastest: a weight tile is read once
+  const int n0 = (tile / m_tiles) * BMW;
+  const int kb0 = (int)((int64_t)nkb * rank / splits);
+  const int kb1 = (int)((int64_t)nkb * (rank + 1) / splits);
+
+  const uint32_t sb = smem_addr(smem);
+  const uint32_t full0 = sb + C::kOffBars;
+  const uint32_t empty0 = full0 + 8 * C::kStages;
+  const uint32_t accum = empty0 + 8 * C::kStages;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kOffTmem);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    aborted = 0;
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(full0 + 8 * s, 1);
+      mbar_init(empty0 + 8 * s, 1);
+    }
+    mbar_init(accum, 1);
+    fence_barrier_init();
+  }
+  if (warp == 1) tmem_alloc(smem_addr(tmem_slot), C::kTmemCols);
+  if (warp == 0 && lane == 0) {
+    prefetch_tensormap(&tm_w);
+    prefetch_tensormap(&tm_x);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+  pdl_launch();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int issued = kb0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        const int i = kb - kb0, s = i % C::kStages;
+        if (!mbar_wait(empty0 + 8 * s, ((i / C::kStages) & 1) ^ 1, status)) {
+          aborted = 1;
+          break;
+        }
+        const uint32_t dst = sb + s * C::kStageBytes;
+        mbar_arrive_expect_tx(full0 + 8 * s, C::kStageBytes);
+        tma_load_2d(dst, &tm_w, kb * BK, n0, full0 + 8 * s);
+        tma_load_2d(dst + kWBytes, &tm_x, kb * BK, m0, full0 + 8 * s);
+        issued = kb + 1;
+      }
+      for (int kb = max(kb0, issued - C::kStages); kb < issued; ++kb) {  // own copies have landed
+        const int i = kb - kb0;
+        mbar_wait(full0 + 8 * (i % C::kStages), (i / C::kStages) & 1, status);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      for (int kb = kb0; kb < kb1; ++kb) {
+        const int i = kb - kb0, s = i % C::kStages;
+        if (!mbar_wait(full0 + 8 * s, (i / C::kStages) & 1, status)) {
+          aborted = 1;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t src = sb + s * C::kStageBytes;
+        const uint64_t da = smem_desc(src), db = smem_desc(src + kWBytes);
+#pragma unroll
+        for (int kk = 0; kk < BK / 32; ++kk)  // +32 bytes along K inside the swizzle atom
+          umma_i8(tmem, da + (uint64_t)(2 * kk), db + (uint64_t)(2 * kk), idesc_i8(BMW, BN),
+                  (i > 0 || kk > 0) ? 1u : 0u);
+        umma_commit(empty0 + 8 * s);
+      }
+      umma_commit(accum);
+    }
+  }
+  __syncwarp();
+  // every warp waits for the accumulator: after it no MMA reads the stages
+  const bool done = mbar_wait(accum, 0, status);
+  if (!done) aborted = 1;
+  tc_fence_after();
+  __syncthreads();
+  const bool ok = !aborted;
+
+  const int q = warp & 3;                 // TMEM lane quarter
+  const int row = 32 * q + lane;
+  const int n = n0 + row;
+  const bool epi = warp >= 2;
+  float ws = 0.f, bias = 0.f;
+  if (epi && n < N) {
+    ws = __ldg(e.weight_scale + n);
+    if (e.bias) bias = ep_f(static_cast<const T*>(e.bias)[n]);
+  }
+  if (splits == 1) {
+    if (epi && ok) {
+#pragma unroll 1
+      for (int c0 = 0; c0 < BN && m0 + c0 < M; c0 += 16) {
+        uint32_t v[16];
+        tmem_ld16(tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)c0, v);
+        const int mc = m0 + c0 + (lane & 15);
+        store_cols<T, 16>(e, v, m0 + c0, M, n, N, ws, bias,
+                          mc < M ? __ldg(e.scale + mc) : 0.f);
+      }
+    }
+  } else {
+    // partial sums [token][weight row] over the (now idle) stages; the token c of the tile is
+    // summed and stored by CTA c % splits
+    int* part = reinterpret_cast<int*>(smem);
+    const int cols = min(BN, M - m0);
+    if (epi) {
+#pragma unroll 1
+      for (int c0 = 0; c0 < cols; c0 += 16) {
+        uint32_t v[16];
+        tmem_ld16(tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)c0, v);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) part[(c0 + j) * BMW + row] = static_cast<int>(v[j]);
+      }
+    }
+    cluster.sync();
+    if (epi && ok) {
+      const T* res = static_cast<const T*>(e.residual);
+      for (int c = rank; c < cols; c += splits) {
+        int sum = 0;
+        for (int r = 0; r < splits; ++r)
+          sum += *cluster.map_shared_rank(part + c * BMW + row, r);
+        const int m = m0 + c;
+        if (n < N) {
+          const int64_t at = (int64_t)m * N + n;
+          float y = fmaf(static_cast<float>(sum), __ldg(e.scale + m) * ws, bias);
+          if (res) y += ep_f(res[at]);
+          static_cast<T*>(e.out)[at] = ep_t<T>(y);
+        }
+      }
+    }
+    cluster.sync();  // the other CTAs have read this one's sums
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, C::kTmemCols);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// pair kernel
+// ---------------------------------------------------------------------------------------------
+
+constexpr int kPairTile = 256;                  // weight rows (both CTAs) and tokens of a tile
+constexpr int kPairStages = 6;
+constexpr int kPairXBytes = 128 * BK;           // this CTA's half of the tokens' operand
+constexpr int kPairStageBytes = kWBytes + kPairXBytes;
+constexpr int kPairOffBars = kPairStages * kPairStageBytes;
+// full[], empty[], acc_full[2], acc_empty[2]
+constexpr int kPairOffTmem = kPairOffBars + (2 * kPairStages + 4) * 8;
+constexpr int kPairSmem = kPairOffTmem + 8 + 1024;
+constexpr int kPairEpiWarps = 8;
+constexpr int kPairThreads = 32 * (2 + kPairEpiWarps);
+constexpr uint32_t kPairTmemCols = 512;         // two accumulators of 256 columns
+constexpr int kPairGroup = 8;                   // weight tiles that run side by side
+static_assert(kPairSmem <= 227 * 1024, "shared memory budget");
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+
+// The address, in the cluster's shared window, of `addr` in the CTA of rank `rank`.
+__device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+
+// Plain load into this CTA's shared memory whose bytes complete on a barrier of the pair's leader.
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, int x, int y,
+                                                 uint32_t leader_bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(leader_bar)
+      : "memory");
+}
+
+__device__ __forceinline__ void umma_i8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                             uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Arrive on the barrier at this offset in both CTAs once the MMAs issued so far have completed.
+__device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+      "[%0], %1;" ::"r"(bar),
+      "h"((uint16_t)3)
+      : "memory");
+}
+
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar)
+               : "memory");
+}
+
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// Tile t of a grid of n_tiles x m_tiles: groups of kPairGroup weight tiles, tokens in the middle,
+// so that the tiles in flight form a near-square block whose operands L2 holds.
+__device__ __forceinline__ void pair_tile(int t, int n_tiles, int m_tiles, int& tn, int& tm) {
+  const int per = kPairGroup * m_tiles;
+  const int g = t / per, r = t - g * per;
+  const int width = min(kPairGroup, n_tiles - g * kPairGroup);
+  tm = r / width;
+  tn = g * kPairGroup + r - tm * width;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kPairThreads, 1)
+    int8_pair_kernel(const __grid_constant__ CUtensorMap tm_w,
+                     const __grid_constant__ CUtensorMap tm_x, const Epilogue e, int M, int N,
+                     int nkb, int n_tiles, int m_tiles, unsigned int* status) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~uintptr_t(1023));
+  __shared__ int aborted;
+  const uint32_t sb = smem_addr(smem);
+  const uint32_t full0 = sb + kPairOffBars;             // leader's: both CTAs' bytes have landed
+  const uint32_t empty0 = full0 + 8 * kPairStages;      // each CTA's: the stage's MMAs are done
+  const uint32_t afull0 = empty0 + 8 * kPairStages;     // each CTA's: an accumulator is complete
+  const uint32_t aempty0 = afull0 + 16;                 // leader's: both CTAs have read it
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + kPairOffTmem);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const int tiles = n_tiles * m_tiles;
+  const int first = blockIdx.x >> 1, stride = gridDim.x >> 1;
+
+  if (threadIdx.x == 0) {
+    aborted = 0;
+    for (int s = 0; s < kPairStages; ++s) {
+      mbar_init(full0 + 8 * s, 1);
+      mbar_init(empty0 + 8 * s, 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(afull0 + 8 * b, 1);
+      mbar_init(aempty0 + 8 * b, 2 * kPairEpiWarps);
+    }
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_addr(tmem_slot)),
+                 "r"(kPairTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  if (warp == 0 && lane == 0) {
+    prefetch_tensormap(&tm_w);
+    prefetch_tensormap(&tm_x);
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_barrier();  // the peer's barriers are initialised too
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+  pdl_launch();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      // both CTAs load their own halves; the bytes of both are counted on the leader's barrier,
+      // which the leader arms.  (The peer may load first: the phase cannot complete before the
+      // leader's arrival, and neither starts a stage before the commit of the MMAs that read it.)
+      int i = 0;
+      bool ok = true;
+      for (int t = first; t < tiles && ok; t += stride) {
+        int tn, tm;
+        pair_tile(t, n_tiles, m_tiles, tn, tm);
+        const int n0 = tn * kPairTile + rank * 128, m0 = tm * kPairTile + rank * 128;
+        for (int kb = 0; kb < nkb; ++kb, ++i) {
+          const int s = i % kPairStages;
+          if (!mbar_wait(empty0 + 8 * s, ((i / kPairStages) & 1) ^ 1, status)) {
+            aborted = 1;
+            ok = false;
+            break;
+          }
+          const uint32_t bar = map_rank(full0 + 8 * s, 0);
+          const uint32_t dst = sb + s * kPairStageBytes;
+          if (rank == 0) mbar_arrive_expect_tx(full0 + 8 * s, 2 * kPairStageBytes);
+          tma_load_2d_pair(dst, &tm_w, kb * BK, n0, bar);
+          tma_load_2d_pair(dst + kWBytes, &tm_x, kb * BK, m0, bar);
+        }
+      }
+      if (!ok) {
+        // the stages in flight land within microseconds; leave them time before the CTA goes
+        const unsigned long long t0 = globaltimer();
+        while (globaltimer() - t0 < 2000000ull) __nanosleep(1000);
+      }
+    }
+  } else if (warp == 1) {
+    if (rank == 0 && lane == 0) {
+      int i = 0, j = 0;
+      bool ok = true;
+      for (int t = first; t < tiles && ok; t += stride, ++j) {
+        const int b = j & 1;
+        if (!mbar_wait(aempty0 + 8 * b, ((j >> 1) & 1) ^ 1, status)) {
+          aborted = 1;
+          break;
+        }
+        tc_fence_after();
+        for (int kb = 0; kb < nkb; ++kb, ++i) {
+          const int s = i % kPairStages;
+          if (!mbar_wait(full0 + 8 * s, (i / kPairStages) & 1, status)) {
+            aborted = 1;
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t src = sb + s * kPairStageBytes;
+          const uint64_t da = smem_desc(src), db = smem_desc(src + kWBytes);
+#pragma unroll
+          for (int kk = 0; kk < BK / 32; ++kk)
+            umma_i8_pair(tmem + b * kPairTile, da + (uint64_t)(2 * kk), db + (uint64_t)(2 * kk),
+                         idesc_i8(2 * BMW, kPairTile), (kb > 0 || kk > 0) ? 1u : 0u);
+          umma_commit_pair(empty0 + 8 * s);
+        }
+        umma_commit_pair(afull0 + 8 * b);
+      }
+    }
+  } else {
+    // epilogue: warp w reads TMEM lanes 32 (w % 4) .. +31; the two warps of a quarter take half of
+    // the columns each
+    const int q = warp & 3, half = (warp - 2) >> 2;
+    const uint32_t leader_empty = map_rank(aempty0, 0);
+    int j = 0;
+    for (int t = first; t < tiles; t += stride, ++j) {
+      const int b = j & 1;
+      int tn, tm;
+      pair_tile(t, n_tiles, m_tiles, tn, tm);
+      const int n = tn * kPairTile + rank * 128 + 32 * q + lane, m0 = tm * kPairTile;
+      float ws = 0.f, bias = 0.f;
+      if (n < N) {
+        ws = __ldg(e.weight_scale + n);
+        if (e.bias) bias = ep_f(static_cast<const T*>(e.bias)[n]);
+      }
+      if (!mbar_wait(afull0 + 8 * b, (j >> 1) & 1, status)) {
+        aborted = 1;
+        break;
+      }
+      tc_fence_after();
+#pragma unroll 1
+      for (int c0 = half * 128; c0 < half * 128 + 128 && m0 + c0 < M; c0 += 32) {
+        uint32_t v[32];
+        tmem_ld32(tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)(b * kPairTile + c0), v);
+        const int mc = m0 + c0 + lane;
+        store_cols<T, 32>(e, v, m0 + c0, M, n, N, ws, bias, mc < M ? __ldg(e.scale + mc) : 0.f);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(leader_empty + 8 * b);
+    }
+  }
+  __syncwarp();
+  // both CTAs are past their last use of either's shared memory and TMEM
+  tc_fence_before();
+  __syncthreads();
+  cluster_barrier();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                 "r"(kPairTmemCols)
+                 : "memory");
+  }
+  __syncthreads();
+  cluster_barrier();
+}
+
+// ---- host --------------------------------------------------------------------------------------
+
+struct Problem {
+  const int8_t* codes;
+  const int8_t* weight;
+  int64_t M, K, N;
+  Epilogue e;
+  unsigned int* status;
+  cudaStream_t stream;
+};
+
+int set_smem(const void* kern, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 64 && ((done.load() >> dev) & 1)) return RW4_OK;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
+    return fail(RW4_ECUDA, "int8_linear: cannot set the kernel's shared memory size");
+  if (dev < 64) done.fetch_or(1ull << dev);
+  return RW4_OK;
+}
+
+int maps(const Problem& p, int box_tokens, CUtensorMap* w, CUtensorMap* x) {
+  int st = make_tensor_map_2d(w, p.weight, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.N, p.K, p.K, BMW,
+                              BK, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (st == RW4_OK)
+    st = make_tensor_map_2d(x, p.codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.M, p.K, p.K,
+                            box_tokens, BK, CU_TENSOR_MAP_SWIZZLE_128B);
+  return st;
+}
+
+int launch(const void* kern, int grid, int threads, int smem, int cluster, cudaStream_t stream,
+           void** args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  const cudaError_t err = cudaLaunchKernelExC(&cfg, kern, args);
+  if (err != cudaSuccess) return cuda_status(err, "rw4 int8_linear launch");
+  return launch_status("rw4 int8_linear launch");
+}
+
+template <int BN, typename T>
+int launch_split(const Problem& p) {
+  using C = SplitCfg<BN>;
+  const void* kern = reinterpret_cast<const void*>(int8_split_kernel<BN, T>);
+  static std::atomic<uint64_t> done{0};
+  int st = set_smem(kern, C::kSmem, done);
+  CUtensorMap w, x;
+  if (st == RW4_OK) st = maps(p, BN, &w, &x);
+  if (st != RW4_OK) return st;
+  int M = (int)p.M, N = (int)p.N, nkb = (int)((p.K + BK - 1) / BK);
+  int m_tiles = (M + BN - 1) / BN;
+  const int64_t tiles = (int64_t)m_tiles * ((N + BMW - 1) / BMW);
+  int splits = 1;
+  while (splits < 8 && tiles * splits * 2 <= (int64_t)sm_count() * C::kCtasPerSm &&
+         nkb / (splits * 2) >= 2)
+    splits *= 2;
+  Epilogue e = p.e;
+  unsigned int* status = p.status;
+  void* args[] = {&w, &x, &e, &M, &N, &nkb, &m_tiles, &status};
+  return launch(kern, (int)(tiles * splits), kSplitThreads, C::kSmem, splits, p.stream, args);
+}
+
+template <typename T>
+int launch_pair(const Problem& p) {
+  const void* kern = reinterpret_cast<const void*>(int8_pair_kernel<T>);
+  static std::atomic<uint64_t> done{0};
+  int st = set_smem(kern, kPairSmem, done);
+  CUtensorMap w, x;
+  if (st == RW4_OK) st = maps(p, 128, &w, &x);
+  if (st != RW4_OK) return st;
+  int M = (int)p.M, N = (int)p.N, nkb = (int)((p.K + BK - 1) / BK);
+  int n_tiles = (N + kPairTile - 1) / kPairTile, m_tiles = (M + kPairTile - 1) / kPairTile;
+  const int64_t tiles = (int64_t)n_tiles * m_tiles;
+  const int64_t pairs = sm_count() / 2;
+  Epilogue e = p.e;
+  unsigned int* status = p.status;
+  void* args[] = {&w, &x, &e, &M, &N, &nkb, &n_tiles, &m_tiles, &status};
+  return launch(kern, 2 * (int)(tiles < pairs ? tiles : pairs), kPairThreads, kPairSmem, 2,
+                p.stream, args);
+}
+
+template <typename T>
+int run(const Problem& p, int32_t path) {
+  const int64_t tiles = ((p.N + kPairTile - 1) / kPairTile) * ((p.M + kPairTile - 1) / kPairTile);
+  const bool pair = path == 2 || (path == 0 && p.M > 256 && tiles >= sm_count() / 2);
+  if (pair) return launch_pair<T>(p);
+  if (p.M <= 16) return launch_split<16, T>(p);
+  if (p.M <= 32) return launch_split<32, T>(p);
+  if (p.M <= 64) return launch_split<64, T>(p);
+  if (p.M <= 128) return launch_split<128, T>(p);
+  return launch_split<256, T>(p);
+}
+
+}  // namespace
+
+extern "C" int rw4_int8_linear(const int8_t* codes, const float* scale, int64_t M, int64_t K,
+                               const int8_t* weight, const float* weight_scale, int64_t N,
+                               const void* bias, const void* residual, void* out,
+                               int32_t out_dtype, int32_t path, void* stream) {
+  using namespace rw4;
+  if (M < 0 || N < 0 || M > (1ll << 30) || N > (1ll << 30))
+    return fail(RW4_EINVAL, "int8_linear: M=%lld N=%lld", (long long)M, (long long)N);
+  if (K < 16 || K % 16 || K > kMaxK)
+    return fail(RW4_EINVAL, "int8_linear: K=%lld (a multiple of 16 from 16 to %lld)", (long long)K,
+                (long long)kMaxK);
+  if (out_dtype != RW4_F32 && out_dtype != RW4_BF16 && out_dtype != RW4_F16)
+    return fail(RW4_EINVAL, "int8_linear: out_dtype %d (0 f32, 1 bf16, 2 f16)", out_dtype);
+  if (path < 0 || path > 2) return fail(RW4_EINVAL, "int8_linear: path %d (0, 1 or 2)", path);
+  // tiles are counted in 32 bits: 128 weight rows x 16 tokens at the smallest, times 8 splits
+  if (((M + 15) / 16) * ((N + 127) / 128) > (1ll << 27))
+    return fail(RW4_EINVAL, "int8_linear: M=%lld x N=%lld is too large for one call", (long long)M,
+                (long long)N);
+  if (M == 0 || N == 0) return RW4_OK;
+  if (!codes || !scale || !weight || !weight_scale || !out)
+    return fail(RW4_EINVAL, "int8_linear: null pointer");
+  if (!aligned(codes, 16) || !aligned(weight, 16))
+    return fail(RW4_EINVAL, "int8_linear: codes and weight must be 16-byte aligned");
+  const int es = out_dtype == RW4_F32 ? 4 : 2;
+  if (!aligned(scale, 4) || !aligned(weight_scale, 4) || !aligned(out, es) || !aligned(bias, es) ||
+      !aligned(residual, es))
+    return fail(RW4_EINVAL, "int8_linear: a pointer is not aligned to its type");
+  Problem p;
+  p.codes = codes;
+  p.weight = weight;
+  p.M = M;
+  p.K = K;
+  p.N = N;
+  p.e = {scale, weight_scale, bias, residual, out};
+  p.status = device_status_ptr();
+  if (!p.status) return fail(RW4_ECUDA, "int8_linear: device status word unavailable");
+  p.stream = as_stream(stream);
+  if (out_dtype == RW4_F32) return run<float>(p, path);
+  if (out_dtype == RW4_F16) return run<__half>(p, path);
+  return run<__nv_bfloat16>(p, path);
+}

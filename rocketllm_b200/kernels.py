@@ -141,6 +141,199 @@ def device_status(clear=True):
     return word.value
 
 
+# ---- 8-bit weights and activations (W8A8) --------------------------------------------------------
+#
+# Rows of signed 8-bit codes with one fp32 scale a row (include/rw4.h).  A projection is
+# quantize -> linear: int8_rmsnorm before q/k/v and gate/up, int8_quantize(up, gate=gate) before
+# down_proj, int8_quantize before o_proj.  These run on the tensors' own device and that device's
+# current stream, allocate only their results, and are forward-only.
+
+_INT8_MAX_K = 131072
+
+
+def _same_device(dev, *tensors):
+    for t in tensors:
+        if t is not None and t.device != dev:
+            raise ValueError(f"tensors on different devices: {dev} and {t.device}")
+
+
+def _int8_call(dev, name, *args):
+    """Call ``name`` with the current stream of ``dev`` as its last argument, on ``dev``."""
+    stream = torch.cuda.current_stream(dev).cuda_stream
+    if torch.cuda.current_device() == dev.index:
+        _lib.call(name, *args, stream)
+    else:
+        with torch.cuda.device(dev):
+            _lib.call(name, *args, stream)
+
+
+def _rows(t, what):
+    """``t [..., K]`` as rows: ``(tensor, element stride between rows)``; a view where one row
+    stride describes ``t``, else a compact copy."""
+    if not t.is_cuda:
+        raise ValueError(f"RW4 kernels take CUDA tensors only (there is no CPU path); {what} is on "
+                         f"{t.device}")
+    if t.dtype not in _DTYPE_CODE:
+        raise TypeError(f"{what} must be float32, bfloat16 or float16, not {t.dtype}")
+    if t.dim() < 1:
+        raise ValueError(f"{what} must have at least one dimension")
+    k = t.shape[-1]
+    if not 1 <= k <= _INT8_MAX_K:
+        raise ValueError(f"{what} has rows of {k} values (1 to {_INT8_MAX_K})")
+    if t.stride(-1) != 1:
+        t = t.contiguous()
+    t = t if t.dim() == 2 else t.reshape(-1, k)
+    return t, t.stride(0)
+
+
+def _codes_out(out, shape, dev):
+    """The ``(codes, scale)`` a row kernel writes: ``out``, checked, or new tensors."""
+    if out is None:
+        return (torch.empty(shape, dtype=torch.int8, device=dev),
+                torch.empty(shape[:-1], dtype=torch.float32, device=dev))
+    codes, scale = out
+    if codes.dtype != torch.int8 or scale.dtype != torch.float32:
+        raise TypeError("out must be (int8 codes, float32 scale)")
+    if codes.shape != shape or scale.shape != shape[:-1]:
+        raise ValueError(f"out has shapes {tuple(codes.shape)} and {tuple(scale.shape)}; rows are "
+                         f"{tuple(shape)}")
+    _require_cuda(codes, scale)
+    _same_device(dev, codes, scale)
+    return codes, scale
+
+
+def _check_codes(codes, scale, what="scale"):
+    _require_cuda(codes, scale)
+    if codes.dtype != torch.int8 or scale.dtype != torch.float32:
+        raise TypeError(f"codes must be int8 and {what} float32, not {codes.dtype} and "
+                        f"{scale.dtype}")
+    if codes.dim() < 1:
+        raise ValueError("codes must have at least one dimension")
+    if scale.shape != codes.shape[:-1] and scale.shape != codes.shape[:-1] + (1,):
+        raise ValueError(f"{what} of shape {tuple(scale.shape)} for codes of shape "
+                         f"{tuple(codes.shape)}: one a row")
+
+
+def int8_quantize(x, gate=None, out=None):
+    """``(codes, scale)`` of the rows of ``x [..., K]``, or of ``silu(gate) * x`` (the MLP's
+    product: ``x`` is ``up``): int8 ``[..., K]`` and float32 ``[...]``.
+
+    Float32, bfloat16 or float16; rows may be strided (halves of a concatenated projection).  In
+    fp32, ``scale = max|y| / 127`` and ``codes = rint(y * (127 / max|y|))``; a row of zeros (or with
+    ``max|y| < 2**-119``) has scale 0, a row that holds a NaN or an infinity scale NaN, both codes
+    0.  ``out``: ``(codes, scale)`` to write instead of new tensors.
+    """
+    x2, ld = _rows(x, "x")
+    dev = x.device
+    g2, gld = None, 0
+    if gate is not None:
+        if gate.shape != x.shape or gate.dtype != x.dtype:
+            raise ValueError(f"gate is {gate.dtype} {tuple(gate.shape)}, x {x.dtype} "
+                             f"{tuple(x.shape)}")
+        g2, gld = _rows(gate, "gate")
+        _same_device(dev, gate)
+    codes, scale = _codes_out(out, x.shape, dev)
+    _int8_call(dev, "rw4_int8_quantize", x2.data_ptr(), ld, g2.data_ptr() if g2 is not None
+               else None, gld, _DTYPE_CODE[x.dtype], x2.shape[0], x2.shape[1], codes.data_ptr(),
+               scale.data_ptr())
+    return codes, scale
+
+
+def int8_dequantize(codes, scale, dtype=torch.bfloat16, out=None):
+    """``codes * scale`` per row in ``dtype`` (float32, bfloat16 or float16)."""
+    _check_codes(codes, scale)
+    dev = codes.device
+    _same_device(dev, scale, out)
+    if out is None:
+        out = torch.empty(codes.shape, dtype=dtype, device=dev)
+    _require_cuda(out)
+    if out.dtype not in _DTYPE_CODE:
+        raise TypeError(f"int8_dequantize writes float32, bfloat16 or float16, not {out.dtype}")
+    if out.shape != codes.shape:
+        raise ValueError(f"out has shape {tuple(out.shape)}, codes {tuple(codes.shape)}")
+    _int8_call(dev, "rw4_int8_dequantize", codes.data_ptr(), scale.data_ptr(), scale.numel(),
+               codes.shape[-1], out.data_ptr(), _DTYPE_CODE[out.dtype])
+    return out
+
+
+def int8_rmsnorm(x, weight, eps, residual=None, out=None, hidden=None):
+    """RMS norm with an 8-bit output: ``(codes, scale)`` of the rows ``h * rsqrt(mean(h^2) + eps) *
+    weight``, with ``h = x``; given ``residual``, ``h = x + residual`` rounded to their type, and
+    ``(codes, scale, h)``.
+
+    The normed row is not rounded before it is quantized (fp32, as :func:`int8_quantize`).
+    ``weight [K]`` has x's type.  ``hidden``: the tensor to write ``h`` to (contiguous; it may be
+    ``x`` or ``residual`` itself).
+    """
+    x2, ld = _rows(x, "x")
+    dev, k = x.device, x.shape[-1]
+    if weight.shape != (k,) or weight.dtype != x.dtype:
+        raise ValueError(f"weight is {weight.dtype} {tuple(weight.shape)}; x has rows of {k} "
+                         f"{x.dtype} values")
+    _require_cuda(weight)
+    _same_device(dev, weight)
+    r2, rld, h = None, 0, None
+    if residual is not None:
+        if residual.shape != x.shape or residual.dtype != x.dtype:
+            raise ValueError(f"residual is {residual.dtype} {tuple(residual.shape)}, x {x.dtype} "
+                             f"{tuple(x.shape)}")
+        r2, rld = _rows(residual, "residual")
+        h = hidden if hidden is not None else torch.empty(x.shape, dtype=x.dtype, device=dev)
+        _require_cuda(h)
+        if h.shape != x.shape or h.dtype != x.dtype:
+            raise ValueError(f"hidden is {h.dtype} {tuple(h.shape)}, x {x.dtype} "
+                             f"{tuple(x.shape)}")
+        _same_device(dev, residual, h)
+    elif hidden is not None:
+        raise ValueError("hidden is written only when a residual is added")
+    codes, scale = _codes_out(out, x.shape, dev)
+    _int8_call(dev, "rw4_int8_rmsnorm", x2.data_ptr(), ld, r2.data_ptr() if r2 is not None
+               else None, rld, weight.data_ptr(), _DTYPE_CODE[x.dtype], x2.shape[0], k, float(eps),
+               h.data_ptr() if h is not None else None, codes.data_ptr(), scale.data_ptr())
+    return (codes, scale) if h is None else (codes, scale, h)
+
+
+def int8_linear(codes, scale, weight, weight_scale, bias=None, residual=None, dtype=torch.bfloat16,
+                out=None, path=None):
+    """``y = (codes * scale) . (weight * weight_scale)^T (+ bias) (+ residual)`` with 8-bit
+    operands: ``codes`` int8 ``[..., K]``, ``scale`` float32 ``[...]``, ``weight`` int8 ``[N, K]``,
+    ``weight_scale`` float32 ``[N]`` or ``[N, 1]``; returns ``[..., N]`` in ``dtype``.
+
+    The integer sums are exact and the rest is fp32, rounded once.  K is a multiple of 16 up to
+    131056, N any number.  ``bias [N]`` and ``residual [..., N]`` have the output's type; ``out``
+    (contiguous) may be ``residual`` itself.  ``path`` forces a kernel (1: one-CTA tiles with K
+    split over clusters, 2: CTA-pair tiles); every path gives the same bits.
+    """
+    _check_codes(codes, scale)
+    _check_codes(weight, weight_scale, "weight_scale")
+    dev, k = codes.device, codes.shape[-1]
+    if weight.dim() != 2 or weight.shape[1] != k:
+        raise ValueError(f"codes have K={k} but the weight is {tuple(weight.shape)}")
+    n = weight.shape[0]
+    shape = codes.shape[:-1] + (n,)
+    if out is None:
+        out = torch.empty(shape, dtype=dtype, device=dev)
+    elif out.shape != shape:
+        raise ValueError(f"out has shape {tuple(out.shape)}, the product {tuple(shape)}")
+    _require_cuda(out)
+    if out.dtype not in _DTYPE_CODE:
+        raise TypeError(f"int8_linear writes float32, bfloat16 or float16, not {out.dtype}")
+    for t, what, want in ((bias, "bias", (n,)), (residual, "residual", tuple(shape))):
+        if t is None:
+            continue
+        if tuple(t.shape) != want or t.dtype != out.dtype:
+            raise ValueError(f"{what} is {t.dtype} {tuple(t.shape)}; it must be {out.dtype} "
+                             f"{want}")
+        _require_cuda(t)
+    _same_device(dev, scale, weight, weight_scale, bias, residual, out)
+    _int8_call(dev, "rw4_int8_linear", codes.data_ptr(), scale.data_ptr(), scale.numel(), k,
+               weight.data_ptr(), weight_scale.data_ptr(), n,
+               bias.data_ptr() if bias is not None else None,
+               residual.data_ptr() if residual is not None else None, out.data_ptr(),
+               _DTYPE_CODE[out.dtype], 0 if path is None else int(path))
+    return out
+
+
 # ---- routed experts ------------------------------------------------------------------------------
 
 def argmax_rows(scores, out=None):
