@@ -5,7 +5,9 @@
 Every .cu / .cpp file in this folder is compiled with
 ``-gencode arch=compute_100a,code=sm_100a -lineinfo -O3`` and linked into
 ``rocketllm_b200/librw4.so`` next to the package, so the library travels with the source tree.
-Rebuilds only when a source or header is newer than the library.
+``binding/rw4_native.cpp`` (the host fast path of the 8-bit operators' Python entry points) is
+compiled against torch's headers and linked into ``rocketllm_b200/_rw4_native.so``, which loads
+``librw4.so`` from its own folder.  Rebuilds only when a source or header is newer than the library.
 """
 import glob
 import os
@@ -16,6 +18,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 PKG = os.path.dirname(HERE)
 ROOT = os.path.dirname(PKG)
 LIB = os.path.join(PKG, "librw4.so")
+NATIVE_SRC = os.path.join(HERE, "binding", "rw4_native.cpp")
+NATIVE = os.path.join(PKG, "_rw4_native.so")
 BUILD_DIR = os.path.join(PKG, "_build")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
@@ -63,7 +67,30 @@ def build(verbose=False, force=False, extra=()):
         if verbose:
             print(" ".join(cmd), flush=True)
         subprocess.run(cmd, check=True)
+    build_native(verbose, force)
     return LIB
+
+
+def build_native(verbose=False, force=False):
+    """``_rw4_native.so``: host C++ only (no device code), against the installed torch."""
+    if not force and not stale(NATIVE, [NATIVE_SRC, os.path.join(ROOT, "include", "rw4.h")]):
+        return
+    import sysconfig
+
+    import torch
+    troot = os.path.dirname(torch.__file__)
+    cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
+    abi = int(torch.compiled_with_cxx11_abi())
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
+           "-I", sysconfig.get_paths()["include"], "-I", os.path.join(troot, "include"),
+           "-I", os.path.join(troot, "include", "torch", "csrc", "api", "include"),
+           "-I", os.path.join(cuda, "include"), "-I", os.path.join(ROOT, "include"),
+           NATIVE_SRC, "-o", NATIVE, "-L", os.path.join(troot, "lib"), "-ltorch_python",
+           "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda", "-L", PKG, "-lrw4",
+           "-Wl,-rpath,$ORIGIN"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.run(cmd, check=True)
 
 
 if __name__ == "__main__":

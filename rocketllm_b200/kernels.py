@@ -11,6 +11,11 @@ import torch
 
 from . import _lib
 
+try:   # host fast path of the 8-bit operators; without it the same calls are made through ctypes
+    from . import _rw4_native as _native
+except ImportError:
+    _native = None
+
 _DTYPE_CODE = {torch.float32: _lib.RW4_F32, torch.bfloat16: _lib.RW4_BF16,
                torch.float16: _lib.RW4_F16}
 
@@ -146,72 +151,104 @@ def device_status(clear=True):
 # Rows of signed 8-bit codes with one fp32 scale a row (include/rw4.h).  A projection is
 # quantize -> linear: int8_rmsnorm before q/k/v and gate/up, int8_quantize(up, gate=gate) before
 # down_proj, int8_quantize before o_proj.  These run on the tensors' own device and that device's
-# current stream, allocate only their results, and are forward-only.
+# current stream, allocate only their results, and are forward-only.  At decode sizes the host's
+# part of a call is as long as the kernel, so the checks below are plain attribute comparisons.
 
 _INT8_MAX_K = 131072
 
 
-def _same_device(dev, *tensors):
-    for t in tensors:
-        if t is not None and t.device != dev:
-            raise ValueError(f"tensors on different devices: {dev} and {t.device}")
-
-
 def _int8_call(dev, name, *args):
-    """Call ``name`` with the current stream of ``dev`` as its last argument, on ``dev``."""
-    stream = torch.cuda.current_stream(dev).cuda_stream
-    if torch.cuda.current_device() == dev.index:
+    """Call ``name`` on device index ``dev`` with its current stream as the last argument."""
+    stream = torch._C._cuda_getCurrentRawStream(dev)
+    if torch._C._cuda_getDevice() == dev:
         _lib.call(name, *args, stream)
     else:
         with torch.cuda.device(dev):
             _lib.call(name, *args, stream)
 
 
+def _on(t, dev, what):
+    """``t`` is a contiguous tensor on device index ``dev`` (else the error that says what is
+    not)."""
+    if t.get_device() != dev:
+        if not t.is_cuda:
+            _require_cuda(t)
+        raise ValueError(f"tensors on different devices: {what} is on {t.device}, not cuda:{dev}")
+    if not t.is_contiguous():
+        raise ValueError(f"RW4 kernels need contiguous tensors; {what} has strides {t.stride()}")
+
+
 def _rows(t, what):
-    """``t [..., K]`` as rows: ``(tensor, element stride between rows)``; a view where one row
-    stride describes ``t``, else a compact copy."""
+    """``t [..., K]`` as rows: ``(tensor [M, K], element stride between rows)``; a view where one
+    row stride describes ``t``, else a compact copy."""
     if not t.is_cuda:
         raise ValueError(f"RW4 kernels take CUDA tensors only (there is no CPU path); {what} is on "
                          f"{t.device}")
     if t.dtype not in _DTYPE_CODE:
         raise TypeError(f"{what} must be float32, bfloat16 or float16, not {t.dtype}")
-    if t.dim() < 1:
-        raise ValueError(f"{what} must have at least one dimension")
-    k = t.shape[-1]
-    if not 1 <= k <= _INT8_MAX_K:
-        raise ValueError(f"{what} has rows of {k} values (1 to {_INT8_MAX_K})")
+    d = t.dim()
+    if not d or not 1 <= t.shape[-1] <= _INT8_MAX_K:
+        raise ValueError(f"{what} of shape {tuple(t.shape)}: rows have 1 to {_INT8_MAX_K} values")
     if t.stride(-1) != 1:
         t = t.contiguous()
-    t = t if t.dim() == 2 else t.reshape(-1, k)
+    if d != 2:
+        t = t.reshape(-1, t.shape[-1])
     return t, t.stride(0)
 
 
-def _codes_out(out, shape, dev):
-    """The ``(codes, scale)`` a row kernel writes: ``out``, checked, or new tensors."""
+def _pair(t, like, what):
+    """``t`` (gate or residual) as rows beside ``like``: its shape, type and device."""
+    if t.shape != like.shape or t.dtype != like.dtype:
+        raise ValueError(f"{what} is {t.dtype} {tuple(t.shape)}, x {like.dtype} "
+                         f"{tuple(like.shape)}")
+    if t.get_device() != like.get_device():
+        raise ValueError(f"tensors on different devices: {what} is on {t.device}, x on "
+                         f"{like.device}")
+    return _rows(t, what)
+
+
+def _codes_out(out, x, dev):
+    """The ``(codes, scale)`` a row kernel writes for ``x``: ``out``, checked, or new tensors."""
+    shape = x.shape
     if out is None:
-        return (torch.empty(shape, dtype=torch.int8, device=dev),
-                torch.empty(shape[:-1], dtype=torch.float32, device=dev))
+        return x.new_empty(shape, dtype=torch.int8), x.new_empty(shape[:-1], dtype=torch.float32)
     codes, scale = out
     if codes.dtype != torch.int8 or scale.dtype != torch.float32:
         raise TypeError("out must be (int8 codes, float32 scale)")
     if codes.shape != shape or scale.shape != shape[:-1]:
         raise ValueError(f"out has shapes {tuple(codes.shape)} and {tuple(scale.shape)}; rows are "
                          f"{tuple(shape)}")
-    _require_cuda(codes, scale)
-    _same_device(dev, codes, scale)
+    _on(codes, dev, "out codes")
+    _on(scale, dev, "out scale")
     return codes, scale
 
 
-def _check_codes(codes, scale, what="scale"):
-    _require_cuda(codes, scale)
+def _check_codes(codes, scale, dev, what):
+    if dev < 0:
+        _require_cuda(codes)
     if codes.dtype != torch.int8 or scale.dtype != torch.float32:
-        raise TypeError(f"codes must be int8 and {what} float32, not {codes.dtype} and "
+        raise TypeError(f"{what} must be int8 codes and a float32 scale, not {codes.dtype} and "
                         f"{scale.dtype}")
-    if codes.dim() < 1:
-        raise ValueError("codes must have at least one dimension")
-    if scale.shape != codes.shape[:-1] and scale.shape != codes.shape[:-1] + (1,):
-        raise ValueError(f"{what} of shape {tuple(scale.shape)} for codes of shape "
-                         f"{tuple(codes.shape)}: one a row")
+    rows = codes.shape[:-1]
+    if not codes.dim() or (scale.shape != rows and scale.shape != rows + (1,)):
+        raise ValueError(f"{what}: a scale of shape {tuple(scale.shape)} for codes of shape "
+                         f"{tuple(codes.shape)} (one a row)")
+    _on(codes, dev, what)
+    _on(scale, dev, what + " scale")
+
+
+def _int8_out(like, shape, dtype, out, dev):
+    """The floating output of a call: ``out``, checked, or a new tensor."""
+    if out is None:
+        if dtype not in _DTYPE_CODE:
+            raise TypeError(f"the output is float32, bfloat16 or float16, not {dtype}")
+        return like.new_empty(shape, dtype=dtype)
+    if out.dtype not in _DTYPE_CODE:
+        raise TypeError(f"the output is float32, bfloat16 or float16, not {out.dtype}")
+    if out.shape != shape:
+        raise ValueError(f"out has shape {tuple(out.shape)}, the result {tuple(shape)}")
+    _on(out, dev, "out")
+    return out
 
 
 def int8_quantize(x, gate=None, out=None):
@@ -223,34 +260,31 @@ def int8_quantize(x, gate=None, out=None):
     ``max|y| < 2**-119``) has scale 0, a row that holds a NaN or an infinity scale NaN, both codes
     0.  ``out``: ``(codes, scale)`` to write instead of new tensors.
     """
+    if _native is not None and out is None:
+        done = _native.int8_quantize(x, gate)
+        if done is not None:
+            return done
     x2, ld = _rows(x, "x")
-    dev = x.device
-    g2, gld = None, 0
+    dev = x.get_device()
+    gp, gld = None, 0
     if gate is not None:
-        if gate.shape != x.shape or gate.dtype != x.dtype:
-            raise ValueError(f"gate is {gate.dtype} {tuple(gate.shape)}, x {x.dtype} "
-                             f"{tuple(x.shape)}")
-        g2, gld = _rows(gate, "gate")
-        _same_device(dev, gate)
-    codes, scale = _codes_out(out, x.shape, dev)
-    _int8_call(dev, "rw4_int8_quantize", x2.data_ptr(), ld, g2.data_ptr() if g2 is not None
-               else None, gld, _DTYPE_CODE[x.dtype], x2.shape[0], x2.shape[1], codes.data_ptr(),
-               scale.data_ptr())
+        g2, gld = _pair(gate, x, "gate")
+        gp = g2.data_ptr()
+    codes, scale = _codes_out(out, x, dev)
+    _int8_call(dev, "rw4_int8_quantize", x2.data_ptr(), ld, gp, gld, _DTYPE_CODE[x.dtype],
+               x2.shape[0], x2.shape[1], codes.data_ptr(), scale.data_ptr())
     return codes, scale
 
 
 def int8_dequantize(codes, scale, dtype=torch.bfloat16, out=None):
     """``codes * scale`` per row in ``dtype`` (float32, bfloat16 or float16)."""
-    _check_codes(codes, scale)
-    dev = codes.device
-    _same_device(dev, scale, out)
-    if out is None:
-        out = torch.empty(codes.shape, dtype=dtype, device=dev)
-    _require_cuda(out)
-    if out.dtype not in _DTYPE_CODE:
-        raise TypeError(f"int8_dequantize writes float32, bfloat16 or float16, not {out.dtype}")
-    if out.shape != codes.shape:
-        raise ValueError(f"out has shape {tuple(out.shape)}, codes {tuple(codes.shape)}")
+    if _native is not None and out is None:
+        done = _native.int8_dequantize(codes, scale, dtype)
+        if done is not None:
+            return done
+    dev = codes.get_device()
+    _check_codes(codes, scale, dev, "codes")
+    out = _int8_out(codes, codes.shape, dtype, out, dev)
     _int8_call(dev, "rw4_int8_dequantize", codes.data_ptr(), scale.data_ptr(), scale.numel(),
                codes.shape[-1], out.data_ptr(), _DTYPE_CODE[out.dtype])
     return out
@@ -265,31 +299,31 @@ def int8_rmsnorm(x, weight, eps, residual=None, out=None, hidden=None):
     ``weight [K]`` has x's type.  ``hidden``: the tensor to write ``h`` to (contiguous; it may be
     ``x`` or ``residual`` itself).
     """
+    if _native is not None and out is None and hidden is None:
+        done = _native.int8_rmsnorm(x, weight, eps, residual)
+        if done is not None:
+            return done
     x2, ld = _rows(x, "x")
-    dev, k = x.device, x.shape[-1]
-    if weight.shape != (k,) or weight.dtype != x.dtype:
+    dev, k = x.get_device(), x2.shape[1]
+    if weight.dtype != x.dtype or weight.dim() != 1 or weight.shape[0] != k:
         raise ValueError(f"weight is {weight.dtype} {tuple(weight.shape)}; x has rows of {k} "
                          f"{x.dtype} values")
-    _require_cuda(weight)
-    _same_device(dev, weight)
-    r2, rld, h = None, 0, None
+    _on(weight, dev, "weight")
+    rp, rld, h, hp = None, 0, None, None
     if residual is not None:
-        if residual.shape != x.shape or residual.dtype != x.dtype:
-            raise ValueError(f"residual is {residual.dtype} {tuple(residual.shape)}, x {x.dtype} "
-                             f"{tuple(x.shape)}")
-        r2, rld = _rows(residual, "residual")
-        h = hidden if hidden is not None else torch.empty(x.shape, dtype=x.dtype, device=dev)
-        _require_cuda(h)
-        if h.shape != x.shape or h.dtype != x.dtype:
+        r2, rld = _pair(residual, x, "residual")
+        rp = r2.data_ptr()
+        h = x.new_empty(x.shape) if hidden is None else hidden
+        if h.dtype != x.dtype or h.shape != x.shape:
             raise ValueError(f"hidden is {h.dtype} {tuple(h.shape)}, x {x.dtype} "
                              f"{tuple(x.shape)}")
-        _same_device(dev, residual, h)
+        _on(h, dev, "hidden")
+        hp = h.data_ptr()
     elif hidden is not None:
         raise ValueError("hidden is written only when a residual is added")
-    codes, scale = _codes_out(out, x.shape, dev)
-    _int8_call(dev, "rw4_int8_rmsnorm", x2.data_ptr(), ld, r2.data_ptr() if r2 is not None
-               else None, rld, weight.data_ptr(), _DTYPE_CODE[x.dtype], x2.shape[0], k, float(eps),
-               h.data_ptr() if h is not None else None, codes.data_ptr(), scale.data_ptr())
+    codes, scale = _codes_out(out, x, dev)
+    _int8_call(dev, "rw4_int8_rmsnorm", x2.data_ptr(), ld, rp, rld, weight.data_ptr(),
+               _DTYPE_CODE[x.dtype], x2.shape[0], k, eps, hp, codes.data_ptr(), scale.data_ptr())
     return (codes, scale) if h is None else (codes, scale, h)
 
 
@@ -304,33 +338,35 @@ def int8_linear(codes, scale, weight, weight_scale, bias=None, residual=None, dt
     (contiguous) may be ``residual`` itself.  ``path`` forces a kernel (1: one-CTA tiles with K
     split over clusters, 2: CTA-pair tiles); every path gives the same bits.
     """
-    _check_codes(codes, scale)
-    _check_codes(weight, weight_scale, "weight_scale")
-    dev, k = codes.device, codes.shape[-1]
+    if _native is not None and out is None and path is None:
+        done = _native.int8_linear(codes, scale, weight, weight_scale, bias, residual, dtype)
+        if done is not None:
+            return done
+    dev = codes.get_device()
+    _check_codes(codes, scale, dev, "codes")
+    _check_codes(weight, weight_scale, dev, "weight")
+    k = codes.shape[-1]
     if weight.dim() != 2 or weight.shape[1] != k:
         raise ValueError(f"codes have K={k} but the weight is {tuple(weight.shape)}")
     n = weight.shape[0]
     shape = codes.shape[:-1] + (n,)
-    if out is None:
-        out = torch.empty(shape, dtype=dtype, device=dev)
-    elif out.shape != shape:
-        raise ValueError(f"out has shape {tuple(out.shape)}, the product {tuple(shape)}")
-    _require_cuda(out)
-    if out.dtype not in _DTYPE_CODE:
-        raise TypeError(f"int8_linear writes float32, bfloat16 or float16, not {out.dtype}")
-    for t, what, want in ((bias, "bias", (n,)), (residual, "residual", tuple(shape))):
-        if t is None:
-            continue
-        if tuple(t.shape) != want or t.dtype != out.dtype:
-            raise ValueError(f"{what} is {t.dtype} {tuple(t.shape)}; it must be {out.dtype} "
-                             f"{want}")
-        _require_cuda(t)
-    _same_device(dev, scale, weight, weight_scale, bias, residual, out)
+    out = _int8_out(codes, shape, dtype, out, dev)
+    bp = rp = None
+    if bias is not None:
+        if bias.dtype != out.dtype or bias.shape != (n,):
+            raise ValueError(f"bias is {bias.dtype} {tuple(bias.shape)}; it must be {out.dtype} "
+                             f"{(n,)}")
+        _on(bias, dev, "bias")
+        bp = bias.data_ptr()
+    if residual is not None:
+        if residual.dtype != out.dtype or residual.shape != shape:
+            raise ValueError(f"residual is {residual.dtype} {tuple(residual.shape)}; it must be "
+                             f"{out.dtype} {tuple(shape)}")
+        _on(residual, dev, "residual")
+        rp = residual.data_ptr()
     _int8_call(dev, "rw4_int8_linear", codes.data_ptr(), scale.data_ptr(), scale.numel(), k,
-               weight.data_ptr(), weight_scale.data_ptr(), n,
-               bias.data_ptr() if bias is not None else None,
-               residual.data_ptr() if residual is not None else None, out.data_ptr(),
-               _DTYPE_CODE[out.dtype], 0 if path is None else int(path))
+               weight.data_ptr(), weight_scale.data_ptr(), n, bp, rp, out.data_ptr(),
+               _DTYPE_CODE[out.dtype], 0 if path is None else path)
     return out
 
 
