@@ -340,6 +340,7 @@ class RocketModel:
         else:
             model = model_or_path
         self.model = model.eval()
+        quant.fuse_rw8_layers(self.model)   # an RW8 Llama's layers; nothing for other models
         self.device = torch.device(device)
         layers = _decoder_layers(model)
         rest, layer_bytes = footprint(model)   # embeddings, final norm, lm_head: resident

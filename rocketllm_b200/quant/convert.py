@@ -6,6 +6,9 @@ with the reference ``quantize(W, axis=1, group_size=64)`` (``rocketllm/quant/kv_
 ``X.weight_scale``, ``X.weight_zero_point``); everything else (embeddings, norms, routers, biases) is
 kept as it is.  The checkpoint's ``config.json`` declares ``quantization_config = {"quant_method":
 "rw4", ...}``, which is what selects the RW4 backend and quantizer at load.
+
+``save_rw8_checkpoint`` does the same for the 8-bit format (``X.weight`` int8, ``X.weight_scale`` fp32
+per output channel, from ``rw4_int8_quantize``); routed experts stay dense there.
 """
 import json
 import os
@@ -14,7 +17,7 @@ import torch
 from torch import nn
 
 from .. import kernels
-from .hf import QUANT_METHOD, RW4Config, _is_stacked_experts
+from .hf import QUANT_METHOD, RW4Config, RW8Config, _is_stacked_experts, rw8_linears
 
 
 def _quantize(w, device):
@@ -55,9 +58,36 @@ def quantize_state_dict(model, device="cuda", modules_to_not_convert=()):
 
 def save_rw4_checkpoint(model, path, device="cuda", modules_to_not_convert=()):
     """Write ``config.json`` + ``model.safetensors`` of the RW4-encoded ``model`` to ``path``."""
+    sd, qcfg = quantize_state_dict(model, device, modules_to_not_convert)
+    return _save(model, path, sd, qcfg)
+
+
+def quantize_state_dict_rw8(model, device="cuda", modules_to_not_convert=()):
+    """``(state_dict, quantization_config)`` of ``model`` with its Linear weights in RW8."""
+    sd = {}
+    for name, module in rw8_linears(model, modules_to_not_convert):
+        w = module.weight.detach().to(device)
+        if w.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+            w = w.float()
+        codes, scale = kernels.int8_quantize(w)
+        if not bool(torch.isfinite(scale).all()):
+            raise ValueError(f"{name}.weight holds a NaN or an infinity")
+        sd[f"{name}.weight"], sd[f"{name}.weight_scale"] = codes.cpu(), scale[:, None].cpu()
+    for pname, param in model.state_dict().items():
+        if pname not in sd:
+            sd[pname] = param.detach().cpu()
+    return sd, RW8Config(modules_to_not_convert=list(modules_to_not_convert)).to_dict()
+
+
+def save_rw8_checkpoint(model, path, device="cuda", modules_to_not_convert=()):
+    """Write ``config.json`` + ``model.safetensors`` of the RW8-encoded ``model`` to ``path``."""
+    sd, qcfg = quantize_state_dict_rw8(model, device, modules_to_not_convert)
+    return _save(model, path, sd, qcfg)
+
+
+def _save(model, path, sd, qcfg):
     from safetensors.torch import save_file
     os.makedirs(path, exist_ok=True)
-    sd, qcfg = quantize_state_dict(model, device, modules_to_not_convert)
     # tied embeddings share storage with lm_head in some models; safetensors refuses aliases
     seen = {}
     for k, v in list(sd.items()):
@@ -75,4 +105,5 @@ def save_rw4_checkpoint(model, path, device="cuda", modules_to_not_convert=()):
     return path
 
 
-__all__ = ["quantize_state_dict", "save_rw4_checkpoint", "QUANT_METHOD"]
+__all__ = ["quantize_state_dict", "save_rw4_checkpoint", "quantize_state_dict_rw8",
+           "save_rw8_checkpoint", "QUANT_METHOD"]

@@ -11,6 +11,9 @@ coalesced placement copies them as stored, ``rocketllm/quant/registry.py:486-501
 Stacked-expert modules (``MixtralExperts`` style: ``gate_up_proj [E, 2I, H]``, ``down_proj
 [E, H, I]``) get RW4 triples for both weights and the model's experts implementation is pointed at
 ``rw4`` in transformers' ``ALL_EXPERTS_FUNCTIONS`` (``integrations/moe.py:432-515``).
+
+``rw8`` is registered in the same way: its ``nn.Linear`` modules become ``RW8Linear`` (routed experts
+stay dense).
 """
 import torch
 from torch import nn
@@ -20,9 +23,10 @@ from transformers.quantizers.auto import (AUTO_QUANTIZATION_CONFIG_MAPPING, AUTO
 from transformers.quantizers.base import HfQuantizer
 from transformers.utils.quantization_config import QuantizationConfigMixin
 
-from .modules import RW4Linear, rw4_experts_forward, rw4_experts_params
+from .modules import RW4Linear, RW8Linear, rw4_experts_forward, rw4_experts_params
 
 QUANT_METHOD = "rw4"
+QUANT_METHOD_RW8 = "rw8"
 
 
 class RW4Config(QuantizationConfigMixin):
@@ -70,6 +74,48 @@ def convert_modules(model, modules_to_not_convert=()):
     return converted
 
 
+class RW8Config(QuantizationConfigMixin):
+    """``{"quant_method": "rw8", "bits": 8, "modules_to_not_convert": [...]}``."""
+
+    def __init__(self, bits=8, modules_to_not_convert=None, **kwargs):
+        if bits != 8:
+            raise ValueError(f"rw8 is 8-bit, got bits={bits}")
+        self.quant_method = QUANT_METHOD_RW8
+        self.bits = bits
+        self.modules_to_not_convert = list(modules_to_not_convert or [])
+
+    def to_dict(self):
+        return {"quant_method": QUANT_METHOD_RW8, "bits": self.bits,
+                "modules_to_not_convert": list(self.modules_to_not_convert)}
+
+
+def rw8_linears(model, modules_to_not_convert=()):
+    """``(name, module)`` of every ``nn.Linear`` the RW8 format stores in 8 bits: not excluded by
+    name, a width the integer product takes, and not an output head whose weight is tied to the
+    embedding (it stays the embedding's)."""
+    skip = tuple(modules_to_not_convert)
+    tied = (model.get_output_embeddings() if hasattr(model, "get_output_embeddings") and
+            getattr(getattr(model, "config", None), "tie_word_embeddings", False) else None)
+    for name, module in list(model.named_modules()):
+        if any(name == s or name.endswith("." + s) or name.startswith(s + ".") for s in skip):
+            continue
+        if isinstance(module, nn.Linear) and module is not tied and \
+                RW8Linear.supports(module.in_features):
+            yield name, module
+
+
+def convert_modules_rw8(model, modules_to_not_convert=()):
+    """Replace every ``nn.Linear`` of :func:`rw8_linears` with an ``RW8Linear``, on whatever device
+    the skeleton lives (normally meta).  Returns the converted names."""
+    converted = []
+    for name, module in rw8_linears(model, modules_to_not_convert):
+        parent_name, _, leaf = name.rpartition(".")
+        parent = model.get_submodule(parent_name) if parent_name else model
+        setattr(parent, leaf, RW8Linear.from_linear(module))
+        converted.append(name)
+    return converted
+
+
 class RW4HfQuantizer(HfQuantizer):
     """Pre-quantized RW4 checkpoints only; packed tensors load verbatim into RW4 modules."""
 
@@ -100,12 +146,24 @@ class RW4HfQuantizer(HfQuantizer):
         return False
 
 
+class RW8HfQuantizer(RW4HfQuantizer):
+    """Pre-quantized RW8 checkpoints only; codes and scales load verbatim into RW8 modules."""
+
+    def _process_model_before_weight_loading(self, model, **kwargs):
+        convert_modules_rw8(model, self.quantization_config.modules_to_not_convert)
+        return model
+
+
 def register():
     """Register config, quantizer and experts function with transformers (idempotent)."""
     if QUANT_METHOD not in AUTO_QUANTIZATION_CONFIG_MAPPING:
         register_quantization_config(QUANT_METHOD)(RW4Config)
     if QUANT_METHOD not in AUTO_QUANTIZER_MAPPING:
         register_quantizer(QUANT_METHOD)(RW4HfQuantizer)
+    if QUANT_METHOD_RW8 not in AUTO_QUANTIZATION_CONFIG_MAPPING:
+        register_quantization_config(QUANT_METHOD_RW8)(RW8Config)
+    if QUANT_METHOD_RW8 not in AUTO_QUANTIZER_MAPPING:
+        register_quantizer(QUANT_METHOD_RW8)(RW8HfQuantizer)
     ALL_EXPERTS_FUNCTIONS._global_mapping[QUANT_METHOD] = rw4_experts_forward
 
 

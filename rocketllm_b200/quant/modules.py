@@ -1,4 +1,4 @@
-"""Modules that hold RW4 weights and compute on them through the C ABI.
+"""Modules that hold RW4 (and RW8) weights and compute on them through the C ABI.
 
 ``RW4Linear`` replaces ``nn.Linear`` (what transformers' attention / MLP / lm_head forwards call,
 e.g. transformers ``models/llama/modeling_llama.py:171-184``); ``rw4_experts_forward`` replaces the
@@ -54,6 +54,71 @@ class RW4Linear(nn.Module):
     def extra_repr(self):
         return (f"in_features={self.in_features}, out_features={self.out_features}, "
                 f"bias={self.bias is not None}, rw4 group {GROUP}")
+
+
+class Int8Rows:
+    """Rows quantized to 8 bits (``codes`` int8 ``[..., K]``, ``scale`` float32 ``[...]``) standing
+    for a tensor of ``dtype``: what a norm or an MLP product hands to the :class:`RW8Linear` modules
+    that read it, quantized once for all of them."""
+
+    __slots__ = ("codes", "scale", "dtype")
+
+    def __init__(self, codes, scale, dtype):
+        self.codes, self.scale, self.dtype = codes, scale, dtype
+
+    @property
+    def shape(self):
+        return self.codes.shape
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    def dequantize(self):
+        return kernels.int8_dequantize(self.codes, self.scale, dtype=self.dtype)
+
+
+class RW8Linear(nn.Module):
+    """``y = x W^T (+ b)`` with ``W [out, in]`` stored as int8 codes and one fp32 scale per output
+    channel; ``x`` is quantized per row on the way in, or comes as :class:`Int8Rows`."""
+
+    def __init__(self, in_features, out_features, bias=False, device=None, dtype=torch.bfloat16):
+        super().__init__()
+        if not self.supports(in_features):
+            raise ValueError(f"RW8Linear needs in_features % 16 == 0 (up to 131056), got "
+                             f"{in_features}")
+        self.in_features = in_features
+        self.out_features = out_features
+        self.weight = _param((out_features, in_features), torch.int8, device)
+        self.weight_scale = _param((out_features, 1), torch.float32, device)
+        self.bias = _param((out_features,), dtype, device) if bias else None
+
+    @staticmethod
+    def supports(in_features):
+        return in_features % 16 == 0 and 0 < in_features <= 131056
+
+    @classmethod
+    def from_linear(cls, linear, device=None):
+        return cls(linear.in_features, linear.out_features, bias=linear.bias is not None,
+                   device=device if device is not None else linear.weight.device,
+                   dtype=linear.weight.dtype if linear.weight.is_floating_point()
+                   else torch.bfloat16)
+
+    def forward(self, x, residual=None):
+        """``residual [..., out]`` (x's type) is added before the one rounding to x's type."""
+        if isinstance(x, Int8Rows):
+            codes, scale = x.codes, x.scale
+        else:
+            codes, scale = kernels.int8_quantize(x)
+        bias = self.bias
+        if bias is not None and bias.dtype != x.dtype:
+            bias = bias.to(x.dtype)
+        return kernels.int8_linear(codes, scale, self.weight, self.weight_scale, bias=bias,
+                                   residual=residual, dtype=x.dtype)
+
+    def extra_repr(self):
+        return (f"in_features={self.in_features}, out_features={self.out_features}, "
+                f"bias={self.bias is not None}, rw8 per channel")
 
 
 def rw4_experts_params(experts, device=None):

@@ -383,7 +383,7 @@ def register_backend(cls):
 
 def _load_backends():
     if not _BACKENDS:
-        from . import rw4  # noqa: F401 - imported for its registration
+        from . import rw4, rw8  # noqa: F401 - imported for their registration
 
 
 def registered_backends():

@@ -1,0 +1,71 @@
+"""Decoder layers of an RW8 Llama in their 8-bit form: what lies between two projections is one
+kernel that ends in 8-bit rows.
+
+Through the transformers modules a layer's norm writes a bf16 row that q, k and v each quantize
+again, and the residual adds and the MLP's product are kernels of their own.  The layer forward here
+keeps the attention module and computes
+
+    int8_rmsnorm                   input_layernorm, quantized once for q, k and v
+    self_attn                      the model's own; o_proj quantizes the attention output
+    int8_rmsnorm(residual)         residual add + post_attention_layernorm, once for gate and up
+    gate_proj, up_proj             8-bit products
+    int8_quantize(up, gate=gate)   act_fn(gate) * up
+    down_proj(residual)            the product with the residual added in its epilogue
+
+Parameters are read at every call, so a streamed layer (whose parameters are views into the engine's
+slots) takes the same path.
+"""
+import types
+
+from .. import kernels
+from .modules import Int8Rows, RW8Linear
+
+
+def _covered(layer):
+    a, m = getattr(layer, "self_attn", None), getattr(layer, "mlp", None)
+    norms = [getattr(layer, n, None) for n in ("input_layernorm", "post_attention_layernorm")]
+    return (all(isinstance(getattr(a, n, None), RW8Linear)
+                for n in ("q_proj", "k_proj", "v_proj", "o_proj")) and
+            all(isinstance(getattr(m, n, None), RW8Linear)
+                for n in ("gate_proj", "up_proj", "down_proj")) and
+            all(getattr(n, "weight", None) is not None and hasattr(n, "variance_epsilon")
+                for n in norms))
+
+
+def fuse_rw8_layers(model):
+    """Give every decoder layer of an RW8 Llama-architecture ``model`` the 8-bit forward above
+    (layers with other modules, and other models, are left as they are).  Returns how many layers
+    have it."""
+    cfg = getattr(model, "config", None)
+    if getattr(cfg, "model_type", None) != "llama" or \
+            getattr(cfg, "hidden_act", None) not in ("silu", "swish"):
+        return 0
+    layers = getattr(getattr(model, "model", None), "layers", ())
+    n = 0
+    for layer in layers:
+        if _covered(layer):
+            layer.forward = types.MethodType(rw8_layer_forward, layer)
+            n += 1
+    return n
+
+
+def _norm(module, x, residual=None):
+    w = module.weight
+    return kernels.int8_rmsnorm(x, w if w.dtype == x.dtype else w.to(x.dtype),
+                                float(module.variance_epsilon), residual=residual)
+
+
+def rw8_layer_forward(self, hidden_states, attention_mask=None, position_ids=None,
+                      past_key_values=None, use_cache=False, position_embeddings=None, **kwargs):
+    """A Llama decoder layer (transformers ``models/llama/modeling_llama.py``) on 8-bit rows."""
+    dtype = hidden_states.dtype
+    codes, scale = _norm(self.input_layernorm, hidden_states)
+    attn, _ = self.self_attn(hidden_states=Int8Rows(codes, scale, dtype),
+                             attention_mask=attention_mask, position_ids=position_ids,
+                             past_key_values=past_key_values, use_cache=use_cache,
+                             position_embeddings=position_embeddings, **kwargs)
+    codes, scale, hidden = _norm(self.post_attention_layernorm, attn, residual=hidden_states)
+    rows = Int8Rows(codes, scale, dtype)
+    m = self.mlp
+    codes, scale = kernels.int8_quantize(m.up_proj(rows), gate=m.gate_proj(rows))
+    return m.down_proj(Int8Rows(codes, scale, dtype), residual=hidden)

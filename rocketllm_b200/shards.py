@@ -447,17 +447,22 @@ class LayerStager:
 
 
 def build_skeleton(root, dtype=torch.bfloat16):
-    """The RW4 ``*ForCausalLM`` of ``root`` on the meta device (no storage allocated)."""
+    """The RW4 (or RW8) ``*ForCausalLM`` of ``root`` on the meta device (no storage allocated)."""
     from transformers import AutoConfig, AutoModelForCausalLM
 
-    from .quant.hf import convert_modules
+    from .quant import fuse_rw8_layers, quant_method_of
+    from .quant.hf import convert_modules, convert_modules_rw8
     config = AutoConfig.from_pretrained(root)
     q = getattr(config, "quantization_config", None)
     skip = (q.get("modules_to_not_convert") if isinstance(q, dict)
             else getattr(q, "modules_to_not_convert", None)) or ()
     with torch.device("meta"):
         model = AutoModelForCausalLM.from_config(config, dtype=dtype)
-    convert_modules(model, skip)
+    if quant_method_of(q) == "rw8":
+        convert_modules_rw8(model, skip)
+        fuse_rw8_layers(model)
+    else:
+        convert_modules(model, skip)
     return model
 
 
