@@ -455,9 +455,8 @@ int rw4_ring_wait_compute(rw4_ring* ring, void* stream);
  * fp32.  A row with a < 2^-119 is stored as scale 0, codes 0; a row that holds a NaN or an
  * infinity as scale NaN, codes 0 (what reads it is NaN).  `dtype` (RW4_F32, RW4_BF16, RW4_F16) is
  * the type of every floating input; row strides are in elements, any value of at least 0 (rows
- * may overlap); codes, hidden and out are contiguous.  1 <= K <= 131072; M = 0 does nothing.  Rows
- * of 16-byte aligned addresses and strides with K a multiple of 8 take vector loads, any others
- * scalar ones.
+ * may overlap); codes, hidden and out are contiguous.  1 <= K <= 131056; M = 0 does nothing.  Any
+ * length and alignment takes wide loads.
  */
 
 /* codes, scale = quantized rows of x[M, K], or of silu(gate) * x when gate is not null

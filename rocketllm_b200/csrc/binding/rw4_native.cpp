@@ -22,7 +22,7 @@
 
 namespace {
 
-constexpr int64_t kMaxRow = 131072;
+constexpr int64_t kMaxRow = 131056;
 
 // A strided CUDA tensor on device `dev` (any device when dev < 0), not a deferred kind.
 bool plain(PyObject* o, int dev) {

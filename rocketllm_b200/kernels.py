@@ -154,7 +154,7 @@ def device_status(clear=True):
 # current stream, allocate only their results, and are forward-only.  At decode sizes the host's
 # part of a call is as long as the kernel, so the checks below are plain attribute comparisons.
 
-_INT8_MAX_K = 131072
+_INT8_MAX_K = 131056
 
 
 def _int8_call(dev, name, *args):

@@ -20,8 +20,9 @@ def status(name, *args):
     ((P, 64, None, 0, 7, 1, 64, P, P, None), "dtype"),
     ((P, 64, None, 0, BF16, -1, 64, P, P, None), "rows"),
     ((P, 64, None, 0, BF16, 1, 0, P, P, None), "values"),
-    ((P, 64, None, 0, BF16, 1, 131073, P, P, None), "values"),
+    ((P, 64, None, 0, BF16, 1, 131057, P, P, None), "values"),
     ((P, 64, None, 0, BF16, 1 << 40, 64, P, P, None), "rows"),
+    ((P, 64, None, 0, BF16, 1 << 27, 1 << 16, P, P, None), "rows"),
     ((None, 64, None, 0, BF16, 1, 64, P, P, None), "null"),
     ((P, 64, None, 0, BF16, 1, 64, None, P, None), "null"),
     ((P, 64, None, 0, BF16, 1, 64, P, None, None), "null"),

@@ -48,7 +48,7 @@ def randn(seed, *shape, dtype=BF):
 
 ROWS = [(1, 1), (1, 8), (3, 7), (5, 65), (300, 33), (2, 4095), (4, 4096), (3, 4104), (3, 5632),
         (2, 8200), (2, 14336), (2, 16384), (2, 16385), (3, 32776), (1, 53248), (2, 65543),
-        (1, 131072)]
+        (1, 131049), (1, 131056), (65, 250), (65, 264), (9, 509), (9, 1017), (7, 1018), (7, 1023)]
 
 
 @pytest.mark.parametrize("dtype", [BF, F16, F32])
@@ -158,6 +158,7 @@ def test_row_layouts(cuda, dtype):
     views = [base[:, :504], base[:, 496:], base[:, 1:801], base[::2, 3:300], base[:1].expand(5, -1),
              base.t(), base[0], base.view(3, 4, 1000), base.view(3, 4, 1000)[:, 1:3, 7:900],
              base.as_strided((9, 64), (8, 1)), base[:0], base[:, 5:6]]
+    views += [base[:, s:s + n] for s in range(1, 9) for n in (600, 601, 604, 33)]
     for v in views:
         codes, scale = kernels.int8_quantize(v)
         c2, s2 = kernels.int8_quantize(v.clone(memory_format=torch.contiguous_format))
@@ -170,6 +171,39 @@ def test_row_layouts(cuda, dtype):
         got = kernels.int8_quantize(v, gate=v)
         want = kernels.int8_quantize(v.contiguous(), gate=v.contiguous())
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+def test_rows_of_every_alignment(cuda, dtype):
+    """Both inputs, the codes and the hidden rows at every offset from a 16-byte boundary; the bytes
+    around the outputs stay as they were."""
+    m, k = 5, 1037
+    for ox, os, oc in ((0, 0, 0), (1, 2, 3), (3, 0, 5), (0, 5, 8), (7, 7, 7), (2, 4, 6), (4, 1, 1)):
+        x = randn(ox, m, k + 40, dtype=dtype)[:, ox:ox + k]
+        second = randn(os + 50, m, k + 24, dtype=dtype)[:, os:os + k]
+        w = randn(oc + 90, k + 16, dtype=dtype)[oc:oc + k]
+        flat = torch.full((m * k + 64,), 77, dtype=torch.int8, device="cuda")
+        codes = flat[16 + oc:16 + oc + m * k].view(m, k)
+        hflat = torch.full((m * k + 64,), 77, dtype=dtype, device="cuda")
+        hidden = hflat[16 + os:16 + os + m * k].view(m, k)
+        out = (codes, torch.empty(m, device="cuda"))
+        kernels.int8_quantize(x, out=out)
+        check_rows(*out, x)
+        kernels.int8_quantize(x, gate=second, out=out)
+        g = second.double()
+        check_rows(*out, g * torch.sigmoid(g) * x.double(), e=2.0 ** -19)
+        kernels.int8_rmsnorm(x, w, 1e-5, residual=second, out=out, hidden=hidden)
+        assert torch.equal(hidden, (x.double() + second.double()).to(dtype))
+        hd = hidden.double()
+        check_rows(*out, hd * torch.rsqrt(hd.square().mean(-1, keepdim=True) + 1e-5) * w.double(),
+                   e=2.0 ** -19)
+        assert (flat[:16 + oc] == 77).all() and (flat[16 + oc + m * k:] == 77).all()
+        assert (hflat[:16 + os] == 77).all() and (hflat[16 + os + m * k:] == 77).all()
+        # and back, from codes and to values at these offsets
+        back = hflat[16 + os:16 + os + m * k].view(m, k)
+        kernels.int8_dequantize(*out, out=back)
+        assert torch.equal(back, (codes.float() * out[1][:, None]).to(dtype))
+        assert (hflat[:16 + os] == 77).all() and (hflat[16 + os + m * k:] == 77).all()
 
 
 def test_given_outputs(cuda):
@@ -455,7 +489,7 @@ def test_refusals(cuda, native, monkeypatch):
         (TypeError, lambda: kernels.int8_quantize(q)),
         (ValueError, lambda: kernels.int8_quantize(x[:, :0])),
         (ValueError, lambda: kernels.int8_quantize(torch.zeros((), device="cuda"))),
-        (ValueError, lambda: kernels.int8_quantize(torch.zeros(1, 131073, device="cuda"))),
+        (ValueError, lambda: kernels.int8_quantize(torch.zeros(1, 131057, device="cuda"))),
         (ValueError, lambda: kernels.int8_quantize(x, gate=x[:, :128])),
         (ValueError, lambda: kernels.int8_quantize(x, gate=x.float())),
         (ValueError, lambda: kernels.int8_quantize(x, gate=x.cpu())),
