@@ -8,12 +8,17 @@
 // and for y:  a = max |y|,  scale = a / 127,  code = rint(y * (127 / a)), ties to even.  y stays in
 // fp32 from the inputs to the code: one rounding, to 8 bits (a module-by-module model rounds the
 // normed row and the product to bf16 first, which costs accuracy and saves nothing here).
-//   - a row whose scale would be subnormal (a < 2^-119) is stored as scale 0 and codes 0: below it
-//     127 / a overflows fp32;
-//   - a row that holds a NaN or an infinity (in y) is stored as scale NaN and codes 0, so that
-//     what reads the row is NaN instead of a finite number.  The maximum is taken over the bit
-//     patterns of |y| as unsigned numbers, where NaN > infinity > every number, so that no
-//     comparison drops a NaN.
+//   - In a norm, rsqrt(..) is one factor r of the whole row: code = rint(h w * (127 / max |h w|)) and
+//     scale = r * max |h w| / 127, so the sum of squares and the maximum are taken in one pass and
+//     joined across the row in one exchange, and no value is multiplied by r.
+//   - A row whose scale would be subnormal (max |y|, or max |h w|, or a, below 2^-119) is stored as
+//     scale 0 and codes 0: below it 127 / a overflows fp32.
+//   - A row that holds a NaN or an infinity is stored as scale NaN and codes 0, so that what reads
+//     the row is NaN instead of a finite number.  The maximum is the NaN-propagating one.
+//   - Rounding to a code is the addition of 1.5 * 2^23 in the fused multiply-add that scales the
+//     value: the sum's low byte is the code in two's complement, rounded once, to even.  (The
+//     conversion instruction runs at a quarter of the rate, on the unit that also serves silu's
+//     exponential and reciprocal: with it, swiglu 2048 x 28672 took 79 us against SWIGLU_US.)
 //
 // Memory-bound: each input is read once, in 16-byte loads, into registers, where the row stays
 // through the reductions (sum of squares, maximum) until its codes are written.  A thread holds NV
@@ -27,23 +32,24 @@
 // none) is read as the two or three aligned 16-byte granules around each vector, shifted together.
 #include <cooperative_groups.h>
 
+#include <atomic>
 #include <climits>
 #include <cstdlib>
 
-#include "rw4_common.cuh"
+#include "rw4_tma.cuh"
 
 namespace cg = cooperative_groups;
 
 namespace {
 
-using rw4::fail;
+using namespace rw4;
 
 constexpr int kMaxThreads = 512;
+constexpr int kWarpThreads = 128;             // of a CTA whose warps hold a row each
 constexpr int kVec = 8;                       // values a thread takes at a time
 // the widest row of rw4_int8_linear; 8 CTAs x 512 threads x 4 vectors of 8 hold it at any alignment
 constexpr int64_t kMaxK = 131056;
-constexpr uint32_t kTinyBits = 0x04000000u;   // 2^-119
-constexpr uint32_t kInfBits = 0x7f800000u;
+constexpr float kTiny = 1.504632769052528e-36f;   // 2^-119
 
 enum Mode { kPlain = 0, kGated = 1, kNorm = 2, kNormRes = 3 };
 
@@ -104,12 +110,6 @@ __device__ __forceinline__ void unpack(const uint4& u, float (&v)[8], __half) {
   }
 }
 
-__device__ __forceinline__ uint32_t code8(float v) {
-  int q;
-  asm("cvt.rni.sat.s8.f32 %0, %1;" : "=r"(q) : "f"(v));
-  return (uint32_t)q & 0xffu;
-}
-
 // Start of a kernel under programmatic dependent launch: the previous grid's writes are waited
 // for, then the next grid may be scheduled (it waits in the same way).
 __device__ __forceinline__ void pdl_enter() {
@@ -117,28 +117,46 @@ __device__ __forceinline__ void pdl_enter() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
-// Sums in a fixed order (the result does not change from run to run).
-__device__ __forceinline__ float warp_sum(float v) {
+// max(top, |a|, |b|), a NaN if any is
+__device__ __forceinline__ float top3(float top, float a, float b) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(top), "f"(a), "f"(b));
+  return r;
+}
+
+__device__ __forceinline__ float top_of(const float (&v)[8], float top) {
 #pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  for (int j = 0; j < 8; j += 2) top = top3(top, v[j], v[j + 1]);
+  return top;
+}
+
+// What the values of a row are reduced to.
+struct RowSums {
+  float top;   // max |y| (a norm's: max |h w|)
+  float ss;    // a norm's sum of squares
+};
+
+// Over a warp, in a fixed order (the result does not change from run to run).  Bit patterns of
+// magnitudes compare as unsigned numbers, a NaN above infinity.
+template <int MODE>
+__device__ __forceinline__ RowSums warp_sums(RowSums v) {
+  v.top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v.top)));
+  if (MODE >= kNorm) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v.ss += __shfl_xor_sync(0xffffffffu, v.ss, o);
+  }
   return v;
 }
 
-__device__ __forceinline__ float block_sum(float v, float* part) {
-  v = warp_sum(v);
+// Over a CTA; `part` holds one entry a warp.  Two calls in a row take different `part`s (a fast
+// warp's next entry must not replace one that a slow warp still reads).
+template <int MODE>
+__device__ __forceinline__ RowSums block_sums(RowSums v, RowSums* part) {
+  v = warp_sums<MODE>(v);
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
   __syncthreads();
-  const int nw = blockDim.x >> 5;
-  return warp_sum((threadIdx.x & 31) < nw ? part[threadIdx.x & 31] : 0.f);
-}
-
-__device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* part) {
-  v = __reduce_max_sync(0xffffffffu, v);
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
-  __syncthreads();
-  const int nw = blockDim.x >> 5;
-  v = (threadIdx.x & 31) < nw ? part[threadIdx.x & 31] : 0u;
-  return __reduce_max_sync(0xffffffffu, v);
+  const int lane = threadIdx.x & 31;
+  return warp_sums<MODE>(lane < (blockDim.x >> 5) ? part[lane] : RowSums{0.f, 0.f});
 }
 
 __device__ __forceinline__ uint4 load_cached(const void* p) {
@@ -211,6 +229,10 @@ struct Held {
       set(v);
     }
   }
+  __device__ __forceinline__ void load_shared(const T* p) {
+#pragma unroll
+    for (int j = 0; j < kQuads; ++j) u[j] = reinterpret_cast<const uint4*>(p)[j];
+  }
   // `aligned`: every vector of this row starts on 16 bytes
   __device__ __forceinline__ void store(T* row, int i, int K, bool aligned) const {
     if (aligned && i >= 0 && i + kVec <= K) {
@@ -231,22 +253,86 @@ __device__ __forceinline__ int shift_of(const T* p) {
   return static_cast<int>(reinterpret_cast<uintptr_t>(p) & 15);
 }
 
-// max of the bit patterns of |v|
-__device__ __forceinline__ uint32_t top_of(const float (&v)[8], uint32_t top) {
+struct RowScale {
+  float scale, inv;
+  bool bad;
+};
+
+// A row's scale, and the factor to its codes.
+template <int MODE>
+__device__ __forceinline__ RowScale row_scale(const RowSums& v, int K, float eps) {
+  const float a = MODE >= kNorm ? rsqrtf(v.ss / static_cast<float>(K) + eps) * v.top : v.top;
+  RowScale r = {0.f, 0.f, !(v.top < INFINITY) || !(a < INFINITY)};
+  if (r.bad) {
+    r.scale = __uint_as_float(0x7fc00000u);
+  } else if (v.top >= kTiny && a >= kTiny) {
+    r.scale = __fdiv_rn(a, 127.f);
+    r.inv = __fdiv_rn(127.f, v.top);
+  }
+  return r;
+}
+
+// The codes of values i .. i+7 of a row of K (i on an 8-byte boundary of the codes).
+__device__ __forceinline__ void store_codes(int8_t* codes, int i, int K, const float (&y)[8],
+                                            const RowScale& r) {
+  uint32_t lo = 0, hi = 0;
+  if (!r.bad) {
+    uint32_t c[8];   // the code in the low byte
 #pragma unroll
-  for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
-  return top;
+    for (int j = 0; j < 8; ++j) c[j] = __float_as_uint(fmaf(y[j], r.inv, 12582912.f));
+    lo = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+    hi = __byte_perm(__byte_perm(c[4], c[5], 0x0040), __byte_perm(c[6], c[7], 0x0040), 0x5410);
+  }
+  if (i >= 0 && i + kVec <= K) {
+    *reinterpret_cast<uint2*>(codes + i) = make_uint2(lo, hi);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kVec; ++j)
+      if (i + j >= 0 && i + j < K)
+        codes[i + j] = static_cast<int8_t>((j < 4 ? lo : hi) >> (8 * (j & 3)));
+  }
+}
+
+// silu(g) * v
+__device__ __forceinline__ float gated(float v, float g) {
+  return v * __fdividef(g, 1.f + __expf(-g));
+}
+
+// Eight values of a row: y (a norm's: h w) and, in a norm, their squares added to ss; `h` becomes
+// the new residual stream.  Positions outside the row hold 0 everywhere and stay 0.
+template <typename T, int MODE>
+__device__ __forceinline__ void combine(Held<T>& h, const Held<T>& second, const Held<T>& weight,
+                                        float (&y)[8], float& ss) {
+  float t[8];
+  h.get(y);
+  if constexpr (MODE == kGated || MODE == kNormRes) {
+    second.get(t);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] = MODE == kGated ? gated(y[j], t[j]) : y[j] + t[j];
+  }
+  if constexpr (MODE == kNormRes) {
+    h.set(y);
+    h.get(y);
+  }
+  if constexpr (MODE >= kNorm) {
+    weight.get(t);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      ss = fmaf(y[j], y[j], ss);
+      y[j] *= t[j];
+    }
+  }
 }
 
 // who holds a row
 enum Kind { kWarp = 0, kBlock = 1, kCluster = 2 };
 
 template <typename T, int MODE, int NV, int KIND>
-__global__ void __launch_bounds__(kMaxThreads, 2) rows_kernel(const RowArgs a) {
-  __shared__ float fpart[16];
-  __shared__ uint32_t upart[16];
-  __shared__ float fjoin;
-  __shared__ uint32_t ujoin;
+__global__ void __launch_bounds__(KIND == kWarp ? kWarpThreads : kMaxThreads,
+                                  KIND == kWarp ? 4 : sizeof(T) == 4 && NV == 4 ? 1 : 2)
+    rows_kernel(const RowArgs a) {
+  __shared__ RowSums part[16];
+  __shared__ RowSums join;
   int rank = 0, parts = 1;
   if constexpr (KIND == kCluster) {
     rank = static_cast<int>(cg::this_cluster().block_rank());
@@ -270,131 +356,152 @@ __global__ void __launch_bounds__(kMaxThreads, 2) rows_kernel(const RowArgs a) {
   const T* weight = static_cast<const T*>(a.weight);
   const int x_shift = shift_of(x - lead);
 
+  constexpr bool kTwo = MODE == kGated || MODE == kNormRes;
+  const int s_shift = kTwo ? shift_of(second - lead) : 0;
+  const int w_shift = MODE >= kNorm ? shift_of(weight - lead) : 0;
+  T* hidden = static_cast<T*>(a.hidden) + row * K;
+  const bool hidden_aligned = MODE == kNormRes && shift_of(hidden - lead) == 0;
+
   pdl_enter();
-  Held<T> h[NV];   // x, or the new residual stream
-#pragma unroll
-  for (int n = 0; n < NV; ++n)
-    if (base + n * step < K) h[n].template load<false>(x, base + n * step, K, x_shift);
-  // a norm's weight, which all rows share: early where registers allow
-  constexpr bool kEarly = MODE >= kNorm && NV * sizeof(T) <= 4;
-  Held<T> wt[kEarly ? NV : 1];
-  const int w_shift = shift_of(weight - lead);
-  if constexpr (kEarly) {
-#pragma unroll
-    for (int n = 0; n < NV; ++n)
-      if (base + n * step < K) wt[n].template load<true>(weight, base + n * step, K, w_shift);
-  }
-  float y[NV][kVec];
-  if constexpr (MODE == kGated || MODE == kNormRes) {
-    const int s_shift = shift_of(second - lead);
-    Held<T> s[NV];
-#pragma unroll
-    for (int n = 0; n < NV; ++n)
-      if (base + n * step < K) s[n].template load<false>(second, base + n * step, K, s_shift);
-    T* hidden = static_cast<T*>(a.hidden) + row * K;
-    const bool hidden_aligned = shift_of(hidden - lead) == 0;
-#pragma unroll
-    for (int n = 0; n < NV; ++n) {
-      const int i = base + n * step;
-      if (i >= K) continue;
-      float v[8], g[8];
-      h[n].get(v);
-      s[n].get(g);
-#pragma unroll
-      for (int j = 0; j < kVec; ++j) {
-        if constexpr (MODE == kGated)
-          // positions outside the row hold 0 in both, and silu(0) * 0 = 0
-          y[n][j] = v[j] * __fdividef(g[j], 1.f + __expf(-g[j]));
-        else
-          v[j] += g[j];
-      }
-      if constexpr (MODE == kNormRes) {
-        h[n].set(v);
-        h[n].store(hidden, i, K, hidden_aligned);
-      }
-    }
-  }
-  if constexpr (MODE >= kNorm) {
-    float ss = 0.f;
-#pragma unroll
-    for (int n = 0; n < NV; ++n) {
-      if (base + n * step >= K) continue;
-      float v[8];
-      h[n].get(v);
-#pragma unroll
-      for (int j = 0; j < kVec; ++j) ss = fmaf(v[j], v[j], ss);
-    }
-    ss = KIND == kWarp ? warp_sum(ss) : block_sum(ss, fpart);
-    if constexpr (KIND == kCluster) {
-      if (threadIdx.x == 0) fjoin = ss;
-      cg::this_cluster().sync();
-      ss = 0.f;
-      for (int r = 0; r < parts; ++r) ss += *cg::this_cluster().map_shared_rank(&fjoin, r);
-    }
-    const float rs = rsqrtf(ss / static_cast<float>(K) + a.eps);
-#pragma unroll
-    for (int n = 0; n < NV; ++n) {
-      const int i = base + n * step;
-      if (i >= K) continue;
-      float w[8];
-      h[n].get(y[n]);
-      if constexpr (kEarly) {
-        wt[n].get(w);
-      } else {
-        wt[0].template load<true>(weight, i, K, w_shift);
-        wt[0].get(w);
-      }
-#pragma unroll
-      for (int j = 0; j < kVec; ++j)
-        // outside the row: 0, not 0 * infinity
-        y[n][j] = i + j >= 0 && i + j < K ? y[n][j] * rs * w[j] : 0.f;
-    }
-  } else if constexpr (MODE == kPlain) {
-#pragma unroll
-    for (int n = 0; n < NV; ++n) h[n].get(y[n]);
-  }
-  uint32_t top = 0;
-#pragma unroll
-  for (int n = 0; n < NV; ++n)
-    if (base + n * step < K) top = top_of(y[n], top);
-  top = KIND == kWarp ? __reduce_max_sync(0xffffffffu, top) : block_max(top, upart);
-  if constexpr (KIND == kCluster) {
-    if (threadIdx.x == 0) ujoin = top;
-    cg::this_cluster().sync();
-    for (int r = 0; r < parts; ++r) top = max(top, *cg::this_cluster().map_shared_rank(&ujoin, r));
-  }
-  const bool bad = top >= kInfBits;
-  const float amax = __uint_as_float(top);
-  float inv = 0.f, scale = 0.f;
-  if (bad) {
-    scale = __uint_as_float(0x7fc00000u);
-  } else if (top >= kTinyBits) {
-    scale = __fdiv_rn(amax, 127.f);
-    inv = __fdiv_rn(127.f, amax);
-  }
-  if (rank == 0 && (KIND == kWarp ? threadIdx.x & 31 : threadIdx.x) == 0) a.scale[row] = scale;
+  Held<T> h[NV], s[kTwo ? NV : 1], w[MODE >= kNorm ? NV : 1];
 #pragma unroll
   for (int n = 0; n < NV; ++n) {
     const int i = base + n * step;
     if (i >= K) continue;
-    uint32_t lo = 0, hi = 0;
-    if (!bad) {
+    h[n].template load<false>(x, i, K, x_shift);
+    if constexpr (kTwo) s[n].template load<false>(second, i, K, s_shift);
+    if constexpr (MODE >= kNorm) w[n].template load<true>(weight, i, K, w_shift);
+  }
+  float y[NV][kVec];
+  RowSums sums = {0.f, 0.f};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        lo |= code8(y[n][j] * inv) << (8 * j);
-        hi |= code8(y[n][j + 4] * inv) << (8 * j);
-      }
+  for (int n = 0; n < NV; ++n) {
+    const int i = base + n * step;
+    if (i >= K) continue;
+    combine<T, MODE>(h[n], s[kTwo ? n : 0], w[MODE >= kNorm ? n : 0], y[n], sums.ss);
+    if constexpr (MODE == kNormRes) h[n].store(hidden, i, K, hidden_aligned);
+    sums.top = top_of(y[n], sums.top);
+  }
+  sums = KIND == kWarp ? warp_sums<MODE>(sums) : block_sums<MODE>(sums, part);
+  if constexpr (KIND == kCluster) {
+    if (threadIdx.x == 0) join = sums;
+    cg::this_cluster().sync();
+    const int lane = threadIdx.x & 31;
+    sums = warp_sums<MODE>(lane < parts ? *cg::this_cluster().map_shared_rank(&join, lane)
+                                        : RowSums{0.f, 0.f});
+  }
+  const RowScale r8 = row_scale<MODE>(sums, K, a.eps);
+  if (rank == 0 && (KIND == kWarp ? threadIdx.x & 31 : threadIdx.x) == 0) a.scale[row] = r8.scale;
+#pragma unroll
+  for (int n = 0; n < NV; ++n)
+    if (base + n * step < K) store_codes(codes, base + n * step, K, y[n], r8);
+  if constexpr (KIND == kCluster) cg::this_cluster().sync();  // all have read the others' sums
+}
+
+// ---- many rows: a ring of rows in shared memory ---------------------------------------------------
+
+constexpr int kRingNV = 4;
+constexpr int kRingStages = 4;       // at most
+constexpr int kRingThreads = 1024;   // at most (64 registers a thread)
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes,
+                                          uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::
+          "r"(dst),
+      "l"(src), "r"(bytes), "r"(bar)
+      : "memory");
+}
+
+// A CTA takes rows blockIdx.x, + gridDim.x, ...; bulk copies fill the stages ahead, a row is read
+// from its stage into registers once and the stage refilled at once, so the next rows stream in
+// under the reductions and stores of this one.  (With a CTA per row each CTA's loads, reductions
+// and stores follow one another, and 40 to 70% of the bandwidth is what is left.)  A norm's weight
+// stays in shared memory.  Rows here are whole 16-byte units at 16-byte addresses.
+template <typename T, int MODE>
+__global__ void __launch_bounds__(kRingThreads, 1)
+    ring_kernel(const RowArgs a, int stages, unsigned int* status) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ uint64_t bars[kRingStages + 1];
+  __shared__ RowSums part[2][32];
+  __shared__ volatile int aborted;
+  constexpr bool kTwo = MODE == kGated || MODE == kNormRes;
+  constexpr int NV = kRingNV;
+  const int K = a.K;
+  const uint32_t row_bytes = static_cast<uint32_t>(K) * sizeof(T);
+  const uint32_t stage_bytes = kTwo ? 2 * row_bytes : row_bytes;
+  uint8_t* ring = smem + (MODE >= kNorm ? row_bytes : 0);
+  const uint32_t bar0 = smem_addr(bars), wbar = bar0 + 8 * kRingStages;
+  const int64_t mine = (a.M - blockIdx.x + gridDim.x - 1) / gridDim.x;   // rows of this CTA
+  if (threadIdx.x == 0) {
+    aborted = 0;
+    for (int s = 0; s <= kRingStages; ++s) mbar_init(bar0 + 8 * s, 1);
+    fence_barrier_init();
+  }
+  __syncthreads();
+  pdl_enter();
+  auto issue = [&](int64_t j) {   // thread 0
+    const int64_t row = blockIdx.x + j * gridDim.x;
+    const int s = static_cast<int>(j % stages);
+    const uint32_t dst = smem_addr(ring) + s * stage_bytes, bar = bar0 + 8 * s;
+    mbar_arrive_expect_tx(bar, stage_bytes);
+    bulk_load(dst, static_cast<const T*>(a.x) + row * a.x_ld, row_bytes, bar);
+    if (kTwo)
+      bulk_load(dst + row_bytes, static_cast<const T*>(a.second) + row * a.second_ld, row_bytes,
+                bar);
+  };
+  if (threadIdx.x == 0) {
+    if (MODE >= kNorm) {
+      mbar_arrive_expect_tx(wbar, row_bytes);
+      bulk_load(smem_addr(smem), a.weight, row_bytes, wbar);
     }
-    if (i >= 0 && i + kVec <= K) {
-      *reinterpret_cast<uint2*>(codes + i) = make_uint2(lo, hi);
-    } else {
+    for (int64_t j = 0; j < stages && j < mine; ++j) issue(j);
+  }
+  if (MODE >= kNorm && !mbar_wait(wbar, 0, status)) aborted = 1;
+  const int base = threadIdx.x * kVec, step = blockDim.x * kVec;
+  int s = 0;
+  uint32_t phase = 0;
+  for (int64_t j = 0; j < mine; ++j) {
+    const int64_t row = blockIdx.x + j * gridDim.x;
+    // (after a wait that ran out the rest of the loop only keeps the barriers in step)
+    if (!aborted && !mbar_wait(bar0 + 8 * s, phase, status)) aborted = 1;
+    const T* xs = reinterpret_cast<const T*>(ring + s * stage_bytes);
+    float y[NV][kVec];
+    RowSums sums = {0.f, 0.f};
 #pragma unroll
-      for (int j = 0; j < kVec; ++j)
-        if (i + j >= 0 && i + j < K)
-          codes[i + j] = static_cast<int8_t>((j < 4 ? lo : hi) >> (8 * (j & 3)));
+    for (int n = 0; n < NV; ++n) {
+      const int i = base + n * step;
+      if (i >= K) continue;
+      Held<T> h, g, w;
+      h.load_shared(xs + i);
+      if constexpr (kTwo) g.load_shared(xs + K + i);
+      if constexpr (MODE >= kNorm) w.load_shared(reinterpret_cast<const T*>(smem) + i);
+      combine<T, MODE>(h, g, w, y[n], sums.ss);
+      if constexpr (MODE == kNormRes)
+        if (!aborted) h.store(static_cast<T*>(a.hidden) + row * K, i, K, true);
+      sums.top = top_of(y[n], sums.top);
+    }
+    // the stage's values are in registers: order these reads before the copy that refills it
+    fence_proxy_async_smem();
+    sums = block_sums<MODE>(sums, part[j & 1]);
+    if (threadIdx.x == 0 && j + stages < mine && !aborted) issue(j + stages);
+    const RowScale r8 = row_scale<MODE>(sums, K, a.eps);
+    if (!aborted) {
+      if (threadIdx.x == 0) a.scale[row] = r8.scale;
+#pragma unroll
+      for (int n = 0; n < NV; ++n)
+        if (base + n * step < K) store_codes(a.codes + row * K, base + n * step, K, y[n], r8);
+    }
+    if (++s == stages) {
+      s = 0;
+      phase ^= 1;
     }
   }
-  if constexpr (KIND == kCluster) cg::this_cluster().sync();  // all have read the others' sums
+  if (aborted) {
+    // leave the copies in flight time to land before the shared memory goes
+    const unsigned long long t0 = globaltimer();
+    while (globaltimer() - t0 < 2000000ull) __nanosleep(1000);
+  }
 }
 
 template <typename T, int MODE, int NV, int KIND>
@@ -417,16 +524,77 @@ int launch_rows(const RowArgs& a, int64_t blocks, int parts, int threads, cudaSt
   return rw4::launch_status("rw4 int8 rows launch");
 }
 
+// Whether the ring takes the call, and its shape: whole 16-byte rows, enough of them for every CTA.
+template <typename T, int MODE>
+bool ring_shape(const RowArgs& a, int& threads, int& stages, int& grid, int& smem) {
+  constexpr int es = sizeof(T);
+  auto whole = [](const void* p, int64_t ld) { return aligned(p, 16) && ld * es % 16 == 0; };
+  const int nvec = a.K / kVec;
+  if (a.K % kVec || nvec <= 128 || nvec > kRingNV * kRingThreads || !whole(a.x, a.x_ld) ||
+      !whole(a.second, a.second_ld) || !aligned(a.weight, 16) || !aligned(a.hidden, 16) ||
+      !aligned(a.codes, 8))
+    return false;
+  threads = ((nvec + kRingNV - 1) / kRingNV + 31) / 32 * 32;
+  const int row = a.K * es, stage = MODE == kGated || MODE == kNormRes ? 2 * row : row;
+  const int fixed = MODE >= kNorm ? row : 0;
+  constexpr int kRoom = 220 * 1024;
+  static const int want = getenv("RW4_RING_S") ? atoi(getenv("RW4_RING_S")) : 2;
+  stages = want;
+  while (stages > 1 && fixed + stages * stage > kRoom) --stages;
+  smem = fixed + stages * stage;
+  if (smem > kRoom) return false;
+  int per_sm = kRingThreads / threads;   // 64 registers a thread
+  if (per_sm > 16) per_sm = 16;
+  while (per_sm > 1 && per_sm * (smem + 2048) > 227 * 1024) --per_sm;
+  const int64_t ctas = static_cast<int64_t>(sm_count()) * per_sm;
+  static const int minrows = getenv("RW4_RING_MIN") ? atoi(getenv("RW4_RING_MIN")) : 2;
+  if (a.M < minrows * ctas) return false;
+  grid = static_cast<int>(ctas);
+  return true;
+}
+
+template <typename T, int MODE>
+int launch_ring(const RowArgs& a, int threads, int stages, int grid, int smem,
+                cudaStream_t stream) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 64 || !((done.load() >> dev) & 1)) {
+    if (cudaFuncSetAttribute(ring_kernel<T, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             220 * 1024) != cudaSuccess)
+      return fail(RW4_ECUDA, "int8 rows: cannot set the kernel's shared memory size");
+    if (dev < 64) done.fetch_or(1ull << dev);
+  }
+  unsigned int* status = device_status_ptr();
+  if (!status) return fail(RW4_ECUDA, "int8 rows: device status word unavailable");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t err = cudaLaunchKernelEx(&cfg, ring_kernel<T, MODE>, a, stages, status);
+  if (err != cudaSuccess) return cuda_status(err, "rw4 int8 rows launch");
+  return launch_status("rw4 int8 rows launch");
+}
+
 template <typename T, int MODE>
 int run_rows(const RowArgs& a, cudaStream_t stream) {
+  int threads, stages, grid, smem;
+  if (ring_shape<T, MODE>(a, threads, stages, grid, smem))
+    return launch_ring<T, MODE>(a, threads, stages, grid, smem, stream);
   // a row's vectors, with one more where it can start inside one
   const bool whole = a.K % kVec == 0 && rw4::aligned(a.codes, kVec);
   const int nvec = whole ? a.K / kVec : (a.K + 2 * (kVec - 1)) / kVec;
   if (nvec <= 128) {   // one warp a row, four rows a CTA
-    const int64_t blocks = (a.M + 3) / 4;
-    if (nvec <= 32) return launch_rows<T, MODE, 1, kWarp>(a, blocks, 1, 128, stream);
-    if (nvec <= 64) return launch_rows<T, MODE, 2, kWarp>(a, blocks, 1, 128, stream);
-    return launch_rows<T, MODE, 4, kWarp>(a, blocks, 1, 128, stream);
+    const int64_t blocks = (a.M + kWarpThreads / 32 - 1) / (kWarpThreads / 32);
+    if (nvec <= 32) return launch_rows<T, MODE, 1, kWarp>(a, blocks, 1, kWarpThreads, stream);
+    if (nvec <= 64) return launch_rows<T, MODE, 2, kWarp>(a, blocks, 1, kWarpThreads, stream);
+    return launch_rows<T, MODE, 4, kWarp>(a, blocks, 1, kWarpThreads, stream);
   }
   auto threads_for = [](int vecs, int nv) { return (((vecs + nv - 1) / nv) + 31) / 32 * 32; };
   static const int forced = getenv("RW4_ROWS_NV") ? atoi(getenv("RW4_ROWS_NV")) : 0;
