@@ -18,7 +18,7 @@
 //   - Rounding to a code is the addition of 1.5 * 2^23 in the fused multiply-add that scales the
 //     value: the sum's low byte is the code in two's complement, rounded once, to even.  (The
 //     conversion instruction runs at a quarter of the rate, on the unit that also serves silu's
-//     exponential and reciprocal: with it, swiglu 2048 x 28672 took 79 us against SWIGLU_US.)
+//     exponential and reciprocal: with it swiglu 8192 x 8192 took 69 us, without it 56.)
 //
 // Memory-bound: each input is read once, in 16-byte loads, into registers, where the row stays
 // through the reductions (sum of squares, maximum) until its codes are written.  A thread holds NV
@@ -34,7 +34,6 @@
 
 #include <atomic>
 #include <climits>
-#include <cstdlib>
 
 #include "rw4_tma.cuh"
 
@@ -401,7 +400,7 @@ __global__ void __launch_bounds__(KIND == kWarp ? kWarpThreads : kMaxThreads,
 // ---- many rows: a ring of rows in shared memory ---------------------------------------------------
 
 constexpr int kRingNV = 4;
-constexpr int kRingStages = 4;       // at most
+constexpr int kRingStages = 2;       // at most
 constexpr int kRingThreads = 1024;   // at most (64 registers a thread)
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes,
@@ -537,18 +536,21 @@ bool ring_shape(const RowArgs& a, int& threads, int& stages, int& grid, int& sme
   threads = ((nvec + kRingNV - 1) / kRingNV + 31) / 32 * 32;
   const int row = a.K * es, stage = MODE == kGated || MODE == kNormRes ? 2 * row : row;
   const int fixed = MODE >= kNorm ? row : 0;
-  constexpr int kRoom = 220 * 1024;
-  static const int want = getenv("RW4_RING_S") ? atoi(getenv("RW4_RING_S")) : 2;
-  stages = want;
-  while (stages > 1 && fixed + stages * stage > kRoom) --stages;
-  smem = fixed + stages * stage;
-  if (smem > kRoom) return false;
   int per_sm = kRingThreads / threads;   // 64 registers a thread
   if (per_sm > 16) per_sm = 16;
-  while (per_sm > 1 && per_sm * (smem + 2048) > 227 * 1024) --per_sm;
+  auto fits = [&](int n) { return 227 * 1024 / (fixed + n * stage + 2048); };
+  // two stages as long as two CTAs an SM hold them (or the one that its threads allow): below that
+  // a second CTA hides more than a second stage (swiglu 2048 x 14336: 31.5 us with two CTAs of one
+  // stage, 34.0 with one of two; norm with residual 8192 x 8192: 73 us with two CTAs of two
+  // stages, 83 with four of one)
+  stages = fits(2) >= (per_sm < 2 ? per_sm : 2) ? 2 : 1;
+  const int f = fits(stages);
+  if (f < 1) return false;
+  if (per_sm > f) per_sm = f;
+  smem = fixed + stages * stage;
   const int64_t ctas = static_cast<int64_t>(sm_count()) * per_sm;
-  static const int minrows = getenv("RW4_RING_MIN") ? atoi(getenv("RW4_RING_MIN")) : 2;
-  if (a.M < minrows * ctas) return false;
+  // below two rows a CTA a CTA per row is faster (1001 x 5632: norm 7.9 us against 6.1)
+  if (a.M < 2 * ctas) return false;
   grid = static_cast<int>(ctas);
   return true;
 }
@@ -561,7 +563,7 @@ int launch_ring(const RowArgs& a, int threads, int stages, int grid, int smem,
   cudaGetDevice(&dev);
   if (dev >= 64 || !((done.load() >> dev) & 1)) {
     if (cudaFuncSetAttribute(ring_kernel<T, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             220 * 1024) != cudaSuccess)
+                             225 * 1024) != cudaSuccess)
       return fail(RW4_ECUDA, "int8 rows: cannot set the kernel's shared memory size");
     if (dev < 64) done.fetch_or(1ull << dev);
   }
@@ -597,23 +599,25 @@ int run_rows(const RowArgs& a, cudaStream_t stream) {
     return launch_rows<T, MODE, 4, kWarp>(a, blocks, 1, kWarpThreads, stream);
   }
   auto threads_for = [](int vecs, int nv) { return (((vecs + nv - 1) / nv) + 31) / 32 * 32; };
-  static const int forced = getenv("RW4_ROWS_NV") ? atoi(getenv("RW4_ROWS_NV")) : 0;
-  if (forced == 2 && nvec <= 2 * kMaxThreads)
-    return launch_rows<T, MODE, 2, kBlock>(a, a.M, 1, threads_for(nvec, 2), stream);
-  if (forced == 4 && nvec <= 4 * kMaxThreads)
-    return launch_rows<T, MODE, 4, kBlock>(a, a.M, 1, threads_for(nvec, 4), stream);
-  if (nvec <= kMaxThreads)
+  // Few long rows: a cluster a row, one vector a thread, where that is faster than one CTA with
+  // more (one row: swiglu of 28672 values 2.7 us against 4.6, of 14336 2.6 against 3.3; quantize of
+  // 14336 2.4 against 1.9).
+  int parts = 1;
+  while (parts < 8 && nvec > parts * kMaxThreads) parts *= 2;
+  if (nvec * (MODE == kPlain ? 1 : 2) > 4 * kMaxThreads && nvec <= parts * kMaxThreads &&
+      a.M * parts <= sm_count())
+    return launch_rows<T, MODE, 1, kCluster>(a, a.M * parts, parts,
+                                             threads_for((nvec + parts - 1) / parts, 1), stream);
+  // With a CTA or less on every SM threads hide latency, beyond it registers do (norm with residual
+  // of 4096 values: 150 rows 2.3 us with one vector a thread, 2.4 with two; 600 rows 6.2 and 5.5).
+  if (nvec <= kMaxThreads && (a.M <= sm_count() || nvec <= kMaxThreads / 2))
     return launch_rows<T, MODE, 1, kBlock>(a, a.M, 1, threads_for(nvec, 1), stream);
   if (nvec <= 2 * kMaxThreads)
     return launch_rows<T, MODE, 2, kBlock>(a, a.M, 1, threads_for(nvec, 2), stream);
   if (nvec <= 4 * kMaxThreads)
     return launch_rows<T, MODE, 4, kBlock>(a, a.M, 1, threads_for(nvec, 4), stream);
-  static const int fnv = getenv("RW4_ROWS_CNV") ? atoi(getenv("RW4_ROWS_CNV")) : 4;
-  int parts = 2;
-  while (parts < 8 && nvec > parts * fnv * kMaxThreads) parts *= 2;
-  if (fnv == 2 && nvec <= parts * 2 * kMaxThreads)
-    return launch_rows<T, MODE, 2, kCluster>(a, a.M * parts, parts,
-                                             threads_for((nvec + parts - 1) / parts, 2), stream);
+  parts = 2;
+  while (parts < 8 && nvec > parts * 4 * kMaxThreads) parts *= 2;
   return launch_rows<T, MODE, 4, kCluster>(a, a.M * parts, parts,
                                            threads_for((nvec + parts - 1) / parts, 4), stream);
 }
