@@ -23,14 +23,10 @@
 //                  epilogue of one tile runs under the MMAs of the next.
 //
 // Every TMA load is a plain per-CTA load.  Every mbarrier wait is bounded (rw4_tma.cuh).
-#include <cooperative_groups.h>
-
 #include <atomic>
 #include <cstdlib>
 
 #include "rw4_tcgen05.cuh"
-
-namespace cg = cooperative_groups;
 
 namespace {
 
@@ -101,6 +97,36 @@ __device__ __forceinline__ void pdl_launch() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+
+// The address, in the cluster's shared window, of `addr` in the CTA of rank `rank`.
+__device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+
+// Copy within the cluster, from this CTA's shared memory to another's, whose barrier counts it.
+__device__ __forceinline__ void bulk_send(uint32_t dst, uint32_t src, uint32_t bytes,
+                                          uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, "
+      "[%3];" ::"r"(dst),
+      "r"(src), "r"(bytes), "r"(bar)
+      : "memory");
+}
+
+__device__ __forceinline__ void cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 // One weight row's share of the epilogue: `count` tokens from m on, sums in v (already in fp32
 // registers' integer form).  Adjacent lanes hold adjacent outputs n, so a warp's store of one token
 // is one run of 32 outputs.
@@ -125,6 +151,57 @@ __device__ __forceinline__ void store_cols(const Epilogue& e, const uint32_t (&v
   }
 }
 
+__device__ __forceinline__ void st_shared(uint32_t addr, uint32_t v) {
+  asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+
+__device__ __forceinline__ void ld_shared8(uint32_t addr, int (&v)[8]) {
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+               : "r"(addr)
+               : "memory");
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+               : "r"(addr + 16)
+               : "memory");
+}
+
+// Eight adjacent outputs of a token from their exact sums, at element `at` of out (and residual);
+// `left`: outputs from there to the end of the row; wide: whole 16-byte units.
+template <typename T>
+__device__ __forceinline__ void store8(const int (&sum)[8], float sx, const float (&ws)[8],
+                                       const float (&bias)[8], const T* res, T* out, int64_t at,
+                                       int left, bool wide) {
+  constexpr int kQuads = sizeof(T) / 2;
+  __align__(16) T r[8];
+  if (res) {
+    if (wide) {
+#pragma unroll
+      for (int j = 0; j < kQuads; ++j)
+        reinterpret_cast<uint4*>(r)[j] = reinterpret_cast<const uint4*>(res + at)[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) r[j] = j < left ? res[at + j] : ep_t<T>(0.f);
+    }
+  }
+  __align__(16) T y[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    float f = fmaf(static_cast<float>(sum[j]), sx * ws[j], bias[j]);
+    if (res) f += ep_f(r[j]);
+    y[j] = ep_t<T>(f);
+  }
+  if (wide) {
+#pragma unroll
+    for (int j = 0; j < kQuads; ++j)
+      reinterpret_cast<uint4*>(out + at)[j] = reinterpret_cast<const uint4*>(y)[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < left) out[at + j] = y[j];
+  }
+}
+
 // ---------------------------------------------------------------------------------------------
 // split kernel
 // ---------------------------------------------------------------------------------------------
@@ -134,43 +211,53 @@ struct SplitCfg {
   static constexpr int kXBytes = BN * BK;
   static constexpr int kStageBytes = kWBytes + kXBytes;
   // up to 64 tokens two CTAs share an SM (one's prologue and epilogue under the other's loads)
-  static constexpr int kStages = BN == 16 ? 6 : BN == 32 ? 5 : BN == 64 ? 4 : BN == 128 ? 6 : 4;
   static constexpr int kCtasPerSm = BN <= 64 ? 2 : 1;
-  static constexpr int kOffBars = kStages * kStageBytes;  // full[], empty[], accum
-  static constexpr int kOffTmem = kOffBars + (2 * kStages + 1) * 8;
+  static constexpr int kStages = BN == 16 ? 5 : BN == 32 ? 4 : BN == 64 ? 3 : BN == 128 ? 5 : 4;
+  // K splits: the partial sums to send lie over the stages, those received beside them
+  static constexpr bool kSplits = BN <= 128;
+  static constexpr int kPartBytes = kSplits ? BN * BMW * 4 : 0;
+  static constexpr int kOffPart = kStages * kStageBytes;
+  static constexpr int kOffBars = kOffPart + kPartBytes;
+  static constexpr int kOffTmem = kOffBars + (2 * kStages + 2) * 8;
   static constexpr int kSmem = kOffTmem + 8 + 1024;
   static constexpr uint32_t kTmemCols = BN < 32 ? 32 : BN;
-  static_assert(BN * BMW * 4 <= kStages * kStageBytes, "partial sums reuse the stages");
-  static_assert(kSmem * kCtasPerSm <= 227 * 1024 - 1024, "shared memory budget");
+  static constexpr int kEpiWarps = BN <= 64 ? 4 : 8;   // four, or four for each half of the columns
+  static constexpr int kThreads = 64 + 32 * kEpiWarps; // TMA, MMA, epilogue
+  static constexpr int kCols = BN / (kEpiWarps / 4);   // columns of an epilogue warp
+  static_assert(BN * BMW * 4 <= kStages * kStageBytes, "the sums fit over the stages");
+  static_assert((kSmem + 1024) * kCtasPerSm <= 228 * 1024, "shared memory budget");
 };
 
-constexpr int kSplitThreads = 192;  // TMA, MMA, 4 epilogue warps
-
 template <int BN, typename T>
-__global__ void __launch_bounds__(kSplitThreads)
+__global__ void __launch_bounds__(SplitCfg<BN>::kThreads)
     int8_split_kernel(const __grid_constant__ CUtensorMap tm_w,
                       const __grid_constant__ CUtensorMap tm_x, const Epilogue e, int M, int N,
-                      int nkb, int m_tiles, unsigned int* status) {
+                      int nkb, int m_tiles, int log_splits, unsigned int* status) {
   using C = SplitCfg<BN>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
   __shared__ int aborted;
-  cg::cluster_group cluster = cg::this_cluster();
-  const int splits = static_cast<int>(cluster.num_blocks());
-  const int rank = static_cast<int>(cluster.block_rank());
-  const int tile = blockIdx.x / splits;
+  __shared__ float sx[BN];                      // the tokens' scales
+  const int splits = 1 << log_splits;
+  const int rank = blockIdx.x & (splits - 1);   // in the cluster: its CTAs are adjacent
+  const int tile = blockIdx.x >> log_splits;
   const int m0 = (tile % m_tiles) * BN;   // tokens fastest: a weight tile is read once
   const int n0 = (tile / m_tiles) * BMW;
-  const int kb0 = (int)((int64_t)nkb * rank / splits);
-  const int kb1 = (int)((int64_t)nkb * (rank + 1) / splits);
+  const int kb0 = (int)((int64_t)nkb * rank >> log_splits);
+  const int kb1 = (int)((int64_t)nkb * (rank + 1) >> log_splits);
 
   const uint32_t sb = smem_addr(smem);
   const uint32_t full0 = sb + C::kOffBars;
   const uint32_t empty0 = full0 + 8 * C::kStages;
   const uint32_t accum = empty0 + 8 * C::kStages;
+  const uint32_t parts = accum + 8;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kOffTmem);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int cols = min(BN, M - m0);
+  // columns of the tile that CTA r of the cluster sums and stores: r, r + splits, ...
+  auto share = [&](int r) { return (cols - r + splits - 1) >> log_splits; };
+  constexpr uint32_t kColBytes = BMW * 4;
 
   if (threadIdx.x == 0) {
     aborted = 0;
@@ -179,7 +266,10 @@ __global__ void __launch_bounds__(kSplitThreads)
       mbar_init(empty0 + 8 * s, 1);
     }
     mbar_init(accum, 1);
+    mbar_init(parts, 1);
     fence_barrier_init();
+    if (C::kSplits && splits > 1 && share(rank) > 0)
+      mbar_arrive_expect_tx(parts, splits * share(rank) * kColBytes);
   }
   if (warp == 1) tmem_alloc(smem_addr(tmem_slot), C::kTmemCols);
   if (warp == 0 && lane == 0) {
@@ -190,9 +280,16 @@ __global__ void __launch_bounds__(kSplitThreads)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  if (C::kSplits && splits > 1) cluster_arrive();   // this CTA's shared memory and barriers are there
   pdl_wait();
   pdl_launch();
 
+  const int q = warp & 3;                 // TMEM lane quarter
+  const bool epi = warp >= 2;
+  // outputs: this thread takes 8 adjacent weight rows of every kTokens-th token
+  const int et = threadIdx.x - 64;
+  const int n8 = n0 + 8 * (et & 15);
+  float ws[8], bias[8];
   if (warp == 0) {
     if (lane == 0) {
       int issued = kb0;
@@ -232,6 +329,15 @@ __global__ void __launch_bounds__(kSplitThreads)
       }
       umma_commit(accum);
     }
+  } else {
+    // under the loads
+    for (int c = threadIdx.x - 64; c < BN; c += 32 * C::kEpiWarps)
+      sx[c] = m0 + c < M ? __ldg(e.scale + m0 + c) : 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      ws[j] = n8 + j < N ? __ldg(e.weight_scale + n8 + j) : 0.f;
+      bias[j] = e.bias && n8 + j < N ? ep_f(static_cast<const T*>(e.bias)[n8 + j]) : 0.f;
+    }
   }
   __syncwarp();
   // every warp waits for the accumulator: after it no MMA reads the stages
@@ -241,57 +347,63 @@ __global__ void __launch_bounds__(kSplitThreads)
   __syncthreads();
   const bool ok = !aborted;
 
-  const int q = warp & 3;                 // TMEM lane quarter
-  const int row = 32 * q + lane;
-  const int n = n0 + row;
-  const bool epi = warp >= 2;
-  float ws = 0.f, bias = 0.f;
-  if (epi && n < N) {
-    ws = __ldg(e.weight_scale + n);
-    if (e.bias) bias = ep_f(static_cast<const T*>(e.bias)[n]);
-  }
-  if (splits == 1) {
-    if (epi && ok) {
+  // The sums, over the (now idle) stages, token by token: sums[slot][weight row].  Token c of the
+  // tile is finished by CTA c % splits of the cluster; the sums are laid out by receiver, slot
+  // (c % splits) * run + c / splits, so that each receiver's part is one run.  (Short loops on
+  // purpose: every launch runs this code once, and straight-line code for 32 columns spent 3 us, a
+  // K-split one 9, waiting for instructions.)
+  const int run = BN >> log_splits;
+  if (epi) {
+    const uint32_t acc = tmem + ((uint32_t)(32 * q) << 16);
+    const uint32_t at = sb + (uint32_t)(32 * q + lane) * 4;
+    const int c_first = ((warp - 2) >> 2) * C::kCols;
 #pragma unroll 1
-      for (int c0 = 0; c0 < BN && m0 + c0 < M; c0 += 16) {
-        uint32_t v[16];
-        tmem_ld16(tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)c0, v);
-        const int mc = m0 + c0 + (lane & 15);
-        store_cols<T, 16>(e, v, m0 + c0, M, n, N, ws, bias,
-                          mc < M ? __ldg(e.scale + mc) : 0.f);
-      }
-    }
-  } else {
-    // partial sums [token][weight row] over the (now idle) stages; the token c of the tile is
-    // summed and stored by CTA c % splits
-    int* part = reinterpret_cast<int*>(smem);
-    const int cols = min(BN, M - m0);
-    if (epi) {
-#pragma unroll 1
-      for (int c0 = 0; c0 < cols; c0 += 16) {
-        uint32_t v[16];
-        tmem_ld16(tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)c0, v);
+    for (int c0 = c_first; c0 < c_first + C::kCols && c0 < cols; c0 += 16) {
+      uint32_t v[16];
+      tmem_ld16(acc + (uint32_t)c0, v);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) part[(c0 + j) * BMW + row] = static_cast<int>(v[j]);
+      for (int j = 0; j < 16; ++j) {
+        const int c = c0 + j;
+        st_shared(at + ((c & (splits - 1)) * run + (c >> log_splits)) * kColBytes, v[j]);
       }
     }
-    cluster.sync();
-    if (epi && ok) {
-      const T* res = static_cast<const T*>(e.residual);
-      for (int c = rank; c < cols; c += splits) {
-        int sum = 0;
-        for (int r = 0; r < splits; ++r)
-          sum += *cluster.map_shared_rank(part + c * BMW + row, r);
-        const int m = m0 + c;
-        if (n < N) {
-          const int64_t at = (int64_t)m * N + n;
-          float y = fmaf(static_cast<float>(sum), __ldg(e.scale + m) * ws, bias);
-          if (res) y += ep_f(res[at]);
-          static_cast<T*>(e.out)[at] = ep_t<T>(y);
-        }
+    if (C::kSplits && splits > 1) fence_proxy_async_smem();  // before the copies that read them
+    asm volatile("bar.sync 1, %0;" ::"r"(32 * C::kEpiWarps) : "memory");
+  }
+  if (C::kSplits && splits > 1) {
+    cluster_wait();               // the other CTAs' barriers are there
+    // each receiver's run (this CTA's own too) in one bulk copy, counted on the receiver's barrier
+    if (epi && et < splits && ok && share(et) > 0)
+      bulk_send(map_rank(sb + C::kOffPart + rank * run * kColBytes, et), sb + et * run * kColBytes,
+                share(et) * kColBytes, map_rank(parts, et));
+  }
+  if (epi && ok && share(rank) > 0 && (!C::kSplits || splits == 1 || mbar_wait(parts, 0, status))) {
+    constexpr int kTokens = 2 * C::kEpiWarps;   // tokens that the epilogue's threads take at a time
+    const uint32_t got = sb + (C::kSplits && splits > 1 ? C::kOffPart : 0) + 32 * (et & 15);
+    const T* res = static_cast<const T*>(e.residual);
+    T* out = static_cast<T*>(e.out);
+    const bool wide = N % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0 &&
+                      (reinterpret_cast<uintptr_t>(res) & 15) == 0;
+#pragma unroll 1
+    for (int t = et >> 4; t < share(rank); t += kTokens) {
+      int sum[8];
+      ld_shared8(got + t * kColBytes, sum);
+#pragma unroll 1
+      for (int r = 1; r < splits; ++r) {
+        int part[8];
+        ld_shared8(got + (r * run + t) * kColBytes, part);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum[j] += part[j];
       }
+      const int c = (t << log_splits) + rank;
+      if (n8 < N)
+        store8<T>(sum, sx[c], ws, bias, res, out, (int64_t)(m0 + c) * N + n8, N - n8, wide);
     }
-    cluster.sync();  // the other CTAs have read this one's sums
+  }
+  if (C::kSplits && splits > 1) {
+    __syncwarp();
+    cluster_arrive();   // what was sent to this CTA is here
+    cluster_wait();     // what this CTA sent has left its shared memory
   }
   tc_fence_before();
   __syncthreads();
@@ -318,19 +430,6 @@ constexpr int kPairThreads = 32 * (2 + kPairEpiWarps);
 constexpr uint32_t kPairTmemCols = 512;         // two accumulators of 256 columns
 constexpr int kPairGroup = 8;                   // weight tiles that run side by side
 static_assert(kPairSmem <= 227 * 1024, "shared memory budget");
-
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-
-// The address, in the cluster's shared window, of `addr` in the CTA of rank `rank`.
-__device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-  return r;
-}
 
 // Plain load into this CTA's shared memory whose bytes complete on a barrier of the pair's leader.
 __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, int x, int y,
@@ -363,11 +462,6 @@ __device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar)
                : "memory");
-}
-
-__device__ __forceinline__ void cluster_barrier() {
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // Tile t of a grid of n_tiles x m_tiles: groups of kPairGroup weight tiles, tokens in the middle,
@@ -425,7 +519,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
-  cluster_barrier();  // the peer's barriers are initialised too
+  cluster_arrive();
+  cluster_wait();  // the peer's barriers are initialised too
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   pdl_wait();
@@ -529,7 +624,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   // both CTAs are past their last use of either's shared memory and TMEM
   tc_fence_before();
   __syncthreads();
-  cluster_barrier();
+  cluster_arrive();
+  cluster_wait();
   if (warp == 1) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem),
@@ -537,7 +633,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                  : "memory");
   }
   __syncthreads();
-  cluster_barrier();
+  cluster_arrive();
+  cluster_wait();
 }
 
 // ---- host --------------------------------------------------------------------------------------
@@ -603,14 +700,16 @@ int launch_split(const Problem& p) {
   int M = (int)p.M, N = (int)p.N, nkb = (int)((p.K + BK - 1) / BK);
   int m_tiles = (M + BN - 1) / BN;
   const int64_t tiles = (int64_t)m_tiles * ((N + BMW - 1) / BMW);
-  int splits = 1;
-  while (splits < 8 && tiles * splits * 2 <= (int64_t)sm_count() * C::kCtasPerSm &&
-         nkb / (splits * 2) >= 2)
-    splits *= 2;
+  int log_splits = 0;
+  while (C::kSplits && log_splits < 3 && (tiles << (log_splits + 1)) <= (int64_t)sm_count() * C::kCtasPerSm &&
+         (nkb >> (log_splits + 1)) >= 2)
+    ++log_splits;
+  if (C::kSplits && getenv("RW4_SPLIT")) log_splits = atoi(getenv("RW4_SPLIT"));
   Epilogue e = p.e;
   unsigned int* status = p.status;
-  void* args[] = {&w, &x, &e, &M, &N, &nkb, &m_tiles, &status};
-  return launch(kern, (int)(tiles * splits), kSplitThreads, C::kSmem, splits, p.stream, args);
+  void* args[] = {&w, &x, &e, &M, &N, &nkb, &m_tiles, &log_splits, &status};
+  return launch(kern, (int)(tiles << log_splits), C::kThreads, C::kSmem, 1 << log_splits, p.stream,
+                args);
 }
 
 template <typename T>
@@ -637,6 +736,14 @@ int run(const Problem& p, int32_t path) {
   const int64_t tiles = ((p.N + kPairTile - 1) / kPairTile) * ((p.M + kPairTile - 1) / kPairTile);
   const bool pair = path == 2 || (path == 0 && p.M > 256 && tiles >= sm_count() / 2);
   if (pair) return launch_pair<T>(p);
+  if (getenv("RW4_BN")) {
+    const int b = atoi(getenv("RW4_BN"));
+    if (b == 16) return launch_split<16, T>(p);
+    if (b == 32) return launch_split<32, T>(p);
+    if (b == 64) return launch_split<64, T>(p);
+    if (b == 128) return launch_split<128, T>(p);
+    if (b == 256) return launch_split<256, T>(p);
+  }
   if (p.M <= 16) return launch_split<16, T>(p);
   if (p.M <= 32) return launch_split<32, T>(p);
   if (p.M <= 64) return launch_split<64, T>(p);
