@@ -14,7 +14,7 @@
 // wide (one 128-byte swizzle atom: four MMAs of K = 32), loaded by TMA through an mbarrier ring; the
 // ends of K, of the weight rows and of the tokens are zero-filled by TMA and never stored.
 //
-//   split kernel   one CTA for 128 weight rows x BN tokens (BN = 16 .. 256), K split over the CTAs
+//   split kernel   one CTA for 128 weight rows x BN tokens (BN = 16 .. 128), K split over the CTAs
 //                  of a cluster when there are fewer tiles than SMs; the integer partial sums meet
 //                  in distributed shared memory (no workspace, no atomics).
 //   pair kernel    two CTAs (cta_group::2) share one 256 x 256 tile: each holds 128 weight rows and
@@ -24,7 +24,6 @@
 //
 // Every TMA load is a plain per-CTA load.  Every mbarrier wait is bounded (rw4_tma.cuh).
 #include <atomic>
-#include <cstdlib>
 
 #include "rw4_tcgen05.cuh"
 
@@ -78,7 +77,7 @@ __device__ __forceinline__ void umma_i8(uint32_t d_tmem, uint64_t a_desc, uint64
       : "memory");
 }
 
-// 16 columns of this warp's 32 lanes, and 32 (tmem_ld32)
+// 16 columns of this warp's 32 lanes
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
@@ -125,30 +124,6 @@ __device__ __forceinline__ void cluster_arrive() {
 }
 __device__ __forceinline__ void cluster_wait() {
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-
-// One weight row's share of the epilogue: `count` tokens from m on, sums in v (already in fp32
-// registers' integer form).  Adjacent lanes hold adjacent outputs n, so a warp's store of one token
-// is one run of 32 outputs.
-template <typename T, int COLS>
-__device__ __forceinline__ void store_cols(const Epilogue& e, const uint32_t (&v)[COLS], int m,
-                                           int M, int n, int N, float ws, float bias, float sx) {
-  const T* res = static_cast<const T*>(e.residual);
-  T* out = static_cast<T*>(e.out) + (int64_t)m * N + n;
-  const bool row = n < N;
-  T r[COLS];
-  if (res) {
-    res += (int64_t)m * N + n;
-#pragma unroll
-    for (int j = 0; j < COLS; ++j) r[j] = row && m + j < M ? res[(int64_t)j * N] : ep_t<T>(0.f);
-  }
-#pragma unroll
-  for (int j = 0; j < COLS; ++j) {
-    const float s = __shfl_sync(0xffffffffu, sx, j) * ws;
-    float y = fmaf(static_cast<float>(static_cast<int>(v[j])), s, bias);
-    if (res) y += ep_f(r[j]);
-    if (row && m + j < M) out[(int64_t)j * N] = ep_t<T>(y);
-  }
 }
 
 __device__ __forceinline__ void st_shared(uint32_t addr, uint32_t v) {
@@ -212,10 +187,9 @@ struct SplitCfg {
   static constexpr int kStageBytes = kWBytes + kXBytes;
   // up to 64 tokens two CTAs share an SM (one's prologue and epilogue under the other's loads)
   static constexpr int kCtasPerSm = BN <= 64 ? 2 : 1;
-  static constexpr int kStages = BN == 16 ? 5 : BN == 32 ? 4 : BN == 64 ? 3 : BN == 128 ? 5 : 4;
+  static constexpr int kStages = BN == 16 ? 5 : BN == 32 ? 4 : BN == 64 ? 3 : 5;
   // K splits: the partial sums to send lie over the stages, those received beside them
-  static constexpr bool kSplits = BN <= 128;
-  static constexpr int kPartBytes = kSplits ? BN * BMW * 4 : 0;
+  static constexpr int kPartBytes = BN * BMW * 4;
   static constexpr int kOffPart = kStages * kStageBytes;
   static constexpr int kOffBars = kOffPart + kPartBytes;
   static constexpr int kOffTmem = kOffBars + (2 * kStages + 2) * 8;
@@ -224,7 +198,7 @@ struct SplitCfg {
   static constexpr int kEpiWarps = BN <= 64 ? 4 : 8;   // four, or four for each half of the columns
   static constexpr int kThreads = 64 + 32 * kEpiWarps; // TMA, MMA, epilogue
   static constexpr int kCols = BN / (kEpiWarps / 4);   // columns of an epilogue warp
-  static_assert(BN * BMW * 4 <= kStages * kStageBytes, "the sums fit over the stages");
+  static_assert(kPartBytes <= kStages * kStageBytes, "the sums fit over the stages");
   static_assert((kSmem + 1024) * kCtasPerSm <= 228 * 1024, "shared memory budget");
 };
 
@@ -268,7 +242,7 @@ __global__ void __launch_bounds__(SplitCfg<BN>::kThreads)
     mbar_init(accum, 1);
     mbar_init(parts, 1);
     fence_barrier_init();
-    if (C::kSplits && splits > 1 && share(rank) > 0)
+    if (splits > 1 && share(rank) > 0)
       mbar_arrive_expect_tx(parts, splits * share(rank) * kColBytes);
   }
   if (warp == 1) tmem_alloc(smem_addr(tmem_slot), C::kTmemCols);
@@ -280,7 +254,7 @@ __global__ void __launch_bounds__(SplitCfg<BN>::kThreads)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  if (C::kSplits && splits > 1) cluster_arrive();   // this CTA's shared memory and barriers are there
+  if (splits > 1) cluster_arrive();   // this CTA's shared memory and barriers are there
   pdl_wait();
   pdl_launch();
 
@@ -367,19 +341,19 @@ __global__ void __launch_bounds__(SplitCfg<BN>::kThreads)
         st_shared(at + ((c & (splits - 1)) * run + (c >> log_splits)) * kColBytes, v[j]);
       }
     }
-    if (C::kSplits && splits > 1) fence_proxy_async_smem();  // before the copies that read them
+    if (splits > 1) fence_proxy_async_smem();  // before the copies that read them
     asm volatile("bar.sync 1, %0;" ::"r"(32 * C::kEpiWarps) : "memory");
   }
-  if (C::kSplits && splits > 1) {
+  if (splits > 1) {
     cluster_wait();               // the other CTAs' barriers are there
     // each receiver's run (this CTA's own too) in one bulk copy, counted on the receiver's barrier
     if (epi && et < splits && ok && share(et) > 0)
       bulk_send(map_rank(sb + C::kOffPart + rank * run * kColBytes, et), sb + et * run * kColBytes,
                 share(et) * kColBytes, map_rank(parts, et));
   }
-  if (epi && ok && share(rank) > 0 && (!C::kSplits || splits == 1 || mbar_wait(parts, 0, status))) {
+  if (epi && ok && share(rank) > 0 && (splits == 1 || mbar_wait(parts, 0, status))) {
     constexpr int kTokens = 2 * C::kEpiWarps;   // tokens that the epilogue's threads take at a time
-    const uint32_t got = sb + (C::kSplits && splits > 1 ? C::kOffPart : 0) + 32 * (et & 15);
+    const uint32_t got = sb + (splits > 1 ? C::kOffPart : 0) + 32 * (et & 15);
     const T* res = static_cast<const T*>(e.residual);
     T* out = static_cast<T*>(e.out);
     const bool wide = N % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0 &&
@@ -400,7 +374,7 @@ __global__ void __launch_bounds__(SplitCfg<BN>::kThreads)
         store8<T>(sum, sx[c], ws, bias, res, out, (int64_t)(m0 + c) * N + n8, N - n8, wide);
     }
   }
-  if (C::kSplits && splits > 1) {
+  if (splits > 1) {
     __syncwarp();
     cluster_arrive();   // what was sent to this CTA is here
     cluster_wait();     // what this CTA sent has left its shared memory
@@ -417,17 +391,18 @@ __global__ void __launch_bounds__(SplitCfg<BN>::kThreads)
 // pair kernel
 // ---------------------------------------------------------------------------------------------
 
-constexpr int kPairTile = 256;                  // weight rows (both CTAs) and tokens of a tile
+constexpr int kPairRows = 256;                  // weight rows of a tile, 128 of each CTA
+constexpr int kPairTokens = 256;                // tokens of a tile: each CTA loads half
+constexpr int kPairStageBytes = kWBytes + kPairTokens / 2 * BK;
 constexpr int kPairStages = 6;
-constexpr int kPairXBytes = 128 * BK;           // this CTA's half of the tokens' operand
-constexpr int kPairStageBytes = kWBytes + kPairXBytes;
-constexpr int kPairOffBars = kPairStages * kPairStageBytes;
+constexpr int kPairEpiWarps = 8;                // four for each half of the columns
+constexpr int kPairOffOut = kPairStages * kPairStageBytes;       // 16 tokens x 32 sums of a warp
+constexpr int kPairOffBars = kPairOffOut + kPairEpiWarps * 16 * 32 * 4;
 // full[], empty[], acc_full[2], acc_empty[2]
 constexpr int kPairOffTmem = kPairOffBars + (2 * kPairStages + 4) * 8;
 constexpr int kPairSmem = kPairOffTmem + 8 + 1024;
-constexpr int kPairEpiWarps = 8;
 constexpr int kPairThreads = 32 * (2 + kPairEpiWarps);
-constexpr uint32_t kPairTmemCols = 512;         // two accumulators of 256 columns
+constexpr uint32_t kPairTmemCols = 2 * kPairTokens;              // two accumulators
 constexpr int kPairGroup = 8;                   // weight tiles that run side by side
 static_assert(kPairSmem <= 227 * 1024, "shared memory budget");
 
@@ -536,7 +511,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       for (int t = first; t < tiles && ok; t += stride) {
         int tn, tm;
         pair_tile(t, n_tiles, m_tiles, tn, tm);
-        const int n0 = tn * kPairTile + rank * 128, m0 = tm * kPairTile + rank * 128;
+        const int n0 = tn * kPairRows + rank * 128, m0 = tm * kPairTokens + rank * (kPairTokens / 2);
         for (int kb = 0; kb < nkb; ++kb, ++i) {
           const int s = i % kPairStages;
           if (!mbar_wait(empty0 + 8 * s, ((i / kPairStages) & 1) ^ 1, status)) {
@@ -580,8 +555,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           const uint64_t da = smem_desc(src), db = smem_desc(src + kWBytes);
 #pragma unroll
           for (int kk = 0; kk < BK / 32; ++kk)
-            umma_i8_pair(tmem + b * kPairTile, da + (uint64_t)(2 * kk), db + (uint64_t)(2 * kk),
-                         idesc_i8(2 * BMW, kPairTile), (kb > 0 || kk > 0) ? 1u : 0u);
+            umma_i8_pair(tmem + b * kPairTokens, da + (uint64_t)(2 * kk), db + (uint64_t)(2 * kk),
+                         idesc_i8(kPairRows, kPairTokens), (kb > 0 || kk > 0) ? 1u : 0u);
           umma_commit_pair(empty0 + 8 * s);
         }
         umma_commit_pair(afull0 + 8 * b);
@@ -589,19 +564,26 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     }
   } else {
     // epilogue: warp w reads TMEM lanes 32 (w % 4) .. +31; the two warps of a quarter take half of
-    // the columns each
+    // the columns each.  Sixteen tokens at a time pass through the warp's own shared memory, so that
+    // a thread holds eight adjacent outputs of a token.
     const int q = warp & 3, half = (warp - 2) >> 2;
     const uint32_t leader_empty = map_rank(aempty0, 0);
+    const uint32_t mine = sb + kPairOffOut + (warp - 2) * (16 * 32 * 4);
+    const T* res = static_cast<const T*>(e.residual);
+    T* out = static_cast<T*>(e.out);
+    const bool wide = N % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0 &&
+                      (reinterpret_cast<uintptr_t>(res) & 15) == 0;
     int j = 0;
     for (int t = first; t < tiles; t += stride, ++j) {
       const int b = j & 1;
       int tn, tm;
       pair_tile(t, n_tiles, m_tiles, tn, tm);
-      const int n = tn * kPairTile + rank * 128 + 32 * q + lane, m0 = tm * kPairTile;
-      float ws = 0.f, bias = 0.f;
-      if (n < N) {
-        ws = __ldg(e.weight_scale + n);
-        if (e.bias) bias = ep_f(static_cast<const T*>(e.bias)[n]);
+      const int n8 = tn * kPairRows + rank * 128 + 32 * q + 8 * (lane & 3), m0 = tm * kPairTokens;
+      float ws[8], bias[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        ws[i] = n8 + i < N ? __ldg(e.weight_scale + n8 + i) : 0.f;
+        bias[i] = e.bias && n8 + i < N ? ep_f(static_cast<const T*>(e.bias)[n8 + i]) : 0.f;
       }
       if (!mbar_wait(afull0 + 8 * b, (j >> 1) & 1, status)) {
         aborted = 1;
@@ -609,11 +591,23 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       }
       tc_fence_after();
 #pragma unroll 1
-      for (int c0 = half * 128; c0 < half * 128 + 128 && m0 + c0 < M; c0 += 32) {
-        uint32_t v[32];
-        tmem_ld32(tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)(b * kPairTile + c0), v);
-        const int mc = m0 + c0 + lane;
-        store_cols<T, 32>(e, v, m0 + c0, M, n, N, ws, bias, mc < M ? __ldg(e.scale + mc) : 0.f);
+      for (int c0 = half * (kPairTokens / 2); c0 < (half + 1) * (kPairTokens / 2) && m0 + c0 < M; c0 += 16) {
+        const int ma = m0 + c0 + (lane >> 2), mb = ma + 8;   // this thread's two tokens
+        const float sa = ma < M ? __ldg(e.scale + ma) : 0.f, sc = mb < M ? __ldg(e.scale + mb) : 0.f;
+        uint32_t v[16];
+        tmem_ld16(tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)(b * kPairTokens + c0), v);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) st_shared(mine + (i * 32 + lane) * 4, v[i]);
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          int sum[8];
+          ld_shared8(mine + ((i * 8 + (lane >> 2)) * 32 + 8 * (lane & 3)) * 4, sum);
+          const int m = i ? mb : ma;
+          if (n8 < N && m < M)
+            store8<T>(sum, i ? sc : sa, ws, bias, res, out, (int64_t)m * N + n8, N - n8, wide);
+        }
+        __syncwarp();   // read before the next tokens' sums are written
       }
       tc_fence_before();
       __syncwarp();
@@ -700,11 +694,17 @@ int launch_split(const Problem& p) {
   int M = (int)p.M, N = (int)p.N, nkb = (int)((p.K + BK - 1) / BK);
   int m_tiles = (M + BN - 1) / BN;
   const int64_t tiles = (int64_t)m_tiles * ((N + BMW - 1) / BMW);
+  // K is split until every SM has a CTA (four stages' worth of K left to each), and once more where
+  // two fit on an SM and that leaves eight: 1 x 4096 x 4096 5.9 us at 128 CTAs (8 stages each), 6.6
+  // at 256 (4 each); 64 x 14336 x 4096 16.6 at 128 (28 each), 15.5 at 256 (14 each).  More CTAs than
+  // fit at once always lost (256 x 4096 x 6144: 96 CTAs 13.1 us, 192 in two waves 22.6).
   int log_splits = 0;
-  while (C::kSplits && log_splits < 3 && (tiles << (log_splits + 1)) <= (int64_t)sm_count() * C::kCtasPerSm &&
-         (nkb >> (log_splits + 1)) >= 2)
-    ++log_splits;
-  if (C::kSplits && getenv("RW4_SPLIT")) log_splits = atoi(getenv("RW4_SPLIT"));
+  auto may = [&](int64_t ctas, int stages) {
+    return log_splits < 3 && (tiles << (log_splits + 1)) <= ctas &&
+           (nkb >> (log_splits + 1)) >= stages;
+  };
+  while (may(sm_count(), 4)) ++log_splits;
+  if (may((int64_t)sm_count() * C::kCtasPerSm, 8)) ++log_splits;
   Epilogue e = p.e;
   unsigned int* status = p.status;
   void* args[] = {&w, &x, &e, &M, &N, &nkb, &m_tiles, &log_splits, &status};
@@ -718,10 +718,10 @@ int launch_pair(const Problem& p) {
   static std::atomic<uint64_t> done{0};
   int st = set_smem(kern, kPairSmem, done);
   CUtensorMap w, x;
-  if (st == RW4_OK) st = maps(p, 128, &w, &x);
+  if (st == RW4_OK) st = maps(p, kPairTokens / 2, &w, &x);
   if (st != RW4_OK) return st;
   int M = (int)p.M, N = (int)p.N, nkb = (int)((p.K + BK - 1) / BK);
-  int n_tiles = (N + kPairTile - 1) / kPairTile, m_tiles = (M + kPairTile - 1) / kPairTile;
+  int n_tiles = (N + kPairRows - 1) / kPairRows, m_tiles = (M + kPairTokens - 1) / kPairTokens;
   const int64_t tiles = (int64_t)n_tiles * m_tiles;
   const int64_t pairs = sm_count() / 2;
   Epilogue e = p.e;
@@ -731,24 +731,20 @@ int launch_pair(const Problem& p) {
                 p.stream, args);
 }
 
+// Which tiles (times of 148 SMs, in us):
+//   up to 64 tokens   one tile of 16, 32 or 64 tokens, the narrowest that holds them
+//   beyond            tiles of 128 tokens where one wave of CTAs takes them (384 x 4096 x 6144, 144
+//                     tiles: 13.4 against 17.0 for pairs), of 64 where even that leaves most SMs idle
+//                     (128 x 2048 x 2048, 16 tiles of 128: 6.1 against 7.6), else CTA pairs
+//                     (512 x 4096 x 6144, 192 tiles: 17.3 against 24.2 in two waves)
 template <typename T>
 int run(const Problem& p, int32_t path) {
-  const int64_t tiles = ((p.N + kPairTile - 1) / kPairTile) * ((p.M + kPairTile - 1) / kPairTile);
-  const bool pair = path == 2 || (path == 0 && p.M > 256 && tiles >= sm_count() / 2);
-  if (pair) return launch_pair<T>(p);
-  if (getenv("RW4_BN")) {
-    const int b = atoi(getenv("RW4_BN"));
-    if (b == 16) return launch_split<16, T>(p);
-    if (b == 32) return launch_split<32, T>(p);
-    if (b == 64) return launch_split<64, T>(p);
-    if (b == 128) return launch_split<128, T>(p);
-    if (b == 256) return launch_split<256, T>(p);
-  }
+  const int64_t rows = (p.N + BMW - 1) / BMW, tiles128 = rows * ((p.M + 127) / 128);
+  if (path == 2 || (path == 0 && p.M > 64 && tiles128 > sm_count())) return launch_pair<T>(p);
   if (p.M <= 16) return launch_split<16, T>(p);
   if (p.M <= 32) return launch_split<32, T>(p);
-  if (p.M <= 64) return launch_split<64, T>(p);
-  if (p.M <= 128) return launch_split<128, T>(p);
-  return launch_split<256, T>(p);
+  if (p.M <= 64 || tiles128 <= 32) return launch_split<64, T>(p);
+  return launch_split<128, T>(p);
 }
 
 }  // namespace
