@@ -141,40 +141,46 @@ __device__ __forceinline__ void ld_shared8(uint32_t addr, int (&v)[8]) {
                : "memory");
 }
 
-// Eight adjacent outputs of a token from their exact sums, at element `at` of out (and residual);
-// `left`: outputs from there to the end of the row; wide: whole 16-byte units.
+__device__ __forceinline__ int ld_shared(uint32_t addr) {
+  int v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+// Eight adjacent values in whole 16-byte units.
+template <typename T>
+struct Eight {
+  static constexpr int kQuads = sizeof(T) / 2;
+  uint4 u[kQuads];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int j = 0; j < kQuads; ++j) u[j] = reinterpret_cast<const uint4*>(p)[j];
+  }
+};
+
+// Eight adjacent outputs from their exact sums and (res) residuals.
 template <typename T>
 __device__ __forceinline__ void store8(const int (&sum)[8], float sx, const float (&ws)[8],
-                                       const float (&bias)[8], const T* res, T* out, int64_t at,
-                                       int left, bool wide) {
-  constexpr int kQuads = sizeof(T) / 2;
-  __align__(16) T r[8];
-  if (res) {
-    if (wide) {
-#pragma unroll
-      for (int j = 0; j < kQuads; ++j)
-        reinterpret_cast<uint4*>(r)[j] = reinterpret_cast<const uint4*>(res + at)[j];
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) r[j] = j < left ? res[at + j] : ep_t<T>(0.f);
-    }
-  }
+                                       const float (&bias)[8], bool res, const Eight<T>& r, T* out) {
+  const T* rv = reinterpret_cast<const T*>(r.u);
   __align__(16) T y[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     float f = fmaf(static_cast<float>(sum[j]), sx * ws[j], bias[j]);
-    if (res) f += ep_f(r[j]);
+    if (res) f += ep_f(rv[j]);
     y[j] = ep_t<T>(f);
   }
-  if (wide) {
 #pragma unroll
-    for (int j = 0; j < kQuads; ++j)
-      reinterpret_cast<uint4*>(out + at)[j] = reinterpret_cast<const uint4*>(y)[j];
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (j < left) out[at + j] = y[j];
-  }
+  for (int j = 0; j < Eight<T>::kQuads; ++j)
+    reinterpret_cast<uint4*>(out)[j] = reinterpret_cast<const uint4*>(y)[j];
+}
+
+// Whether every output row is whole 16-byte units.  Where it is, a thread stores eight adjacent
+// outputs at a time; else adjacent threads store adjacent outputs (eight single stores of a thread,
+// 16 bytes apart from its neighbour's, took 254 us for 4086 x 5072 x 8212 against 151).
+inline bool wide_rows(const Epilogue& e, int64_t N) {
+  return N % 8 == 0 && ((reinterpret_cast<uintptr_t>(e.out) |
+                         reinterpret_cast<uintptr_t>(e.residual)) & 15) == 0;
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -202,7 +208,7 @@ struct SplitCfg {
   static_assert((kSmem + 1024) * kCtasPerSm <= 228 * 1024, "shared memory budget");
 };
 
-template <int BN, typename T>
+template <int BN, typename T, bool WIDE, bool RES>
 __global__ void __launch_bounds__(SplitCfg<BN>::kThreads)
     int8_split_kernel(const __grid_constant__ CUtensorMap tm_w,
                       const __grid_constant__ CUtensorMap tm_x, const Epilogue e, int M, int N,
@@ -260,9 +266,9 @@ __global__ void __launch_bounds__(SplitCfg<BN>::kThreads)
 
   const int q = warp & 3;                 // TMEM lane quarter
   const bool epi = warp >= 2;
-  // outputs: this thread takes 8 adjacent weight rows of every kTokens-th token
+  // outputs: this thread takes 8 adjacent weight rows of a token (wide), or rows 32 apart
   const int et = threadIdx.x - 64;
-  const int n8 = n0 + 8 * (et & 15);
+  const int n_first = n0 + (WIDE ? 8 * (et & 15) : lane), n_step = WIDE ? 1 : 32;
   float ws[8], bias[8];
   if (warp == 0) {
     if (lane == 0) {
@@ -309,8 +315,9 @@ __global__ void __launch_bounds__(SplitCfg<BN>::kThreads)
       sx[c] = m0 + c < M ? __ldg(e.scale + m0 + c) : 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      ws[j] = n8 + j < N ? __ldg(e.weight_scale + n8 + j) : 0.f;
-      bias[j] = e.bias && n8 + j < N ? ep_f(static_cast<const T*>(e.bias)[n8 + j]) : 0.f;
+      const int n = n_first + j * n_step;
+      ws[j] = n < N ? __ldg(e.weight_scale + n) : 0.f;
+      bias[j] = e.bias && n < N ? ep_f(static_cast<const T*>(e.bias)[n]) : 0.f;
     }
   }
   __syncwarp();
@@ -352,26 +359,61 @@ __global__ void __launch_bounds__(SplitCfg<BN>::kThreads)
                 share(et) * kColBytes, map_rank(parts, et));
   }
   if (epi && ok && share(rank) > 0 && (splits == 1 || mbar_wait(parts, 0, status))) {
-    constexpr int kTokens = 2 * C::kEpiWarps;   // tokens that the epilogue's threads take at a time
-    const uint32_t got = sb + (splits > 1 ? C::kOffPart : 0) + 32 * (et & 15);
+    const uint32_t got = sb + (splits > 1 ? C::kOffPart : 0);
     const T* res = static_cast<const T*>(e.residual);
     T* out = static_cast<T*>(e.out);
-    const bool wide = N % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0 &&
-                      (reinterpret_cast<uintptr_t>(res) & 15) == 0;
+    // (a token's residuals are loaded while the one before it is finished)
+    auto at = [&](int t) { return (int64_t)(m0 + (t << log_splits) + rank) * N + n_first; };
+    if constexpr (WIDE) {
+      constexpr int kTokens = 2 * C::kEpiWarps;
+      const bool mine = n_first < N;
+      int t = et >> 4;
+      Eight<T> r = {}, next = {};
+      if (RES && mine && t < share(rank)) next.load(res + at(t));
 #pragma unroll 1
-    for (int t = et >> 4; t < share(rank); t += kTokens) {
-      int sum[8];
-      ld_shared8(got + t * kColBytes, sum);
+      for (; t < share(rank); t += kTokens) {
+        r = next;
+        if (RES && mine && t + kTokens < share(rank)) next.load(res + at(t + kTokens));
+        const uint32_t from = got + t * kColBytes + 32 * (et & 15);
+        int sum[8];
+        ld_shared8(from, sum);
 #pragma unroll 1
-      for (int r = 1; r < splits; ++r) {
-        int part[8];
-        ld_shared8(got + (r * run + t) * kColBytes, part);
+        for (int k = 1; k < splits; ++k) {
+          int part[8];
+          ld_shared8(from + k * run * kColBytes, part);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sum[j] += part[j];
+          for (int j = 0; j < 8; ++j) sum[j] += part[j];
+        }
+        if (mine)
+          store8<T>(sum, sx[(t << log_splits) + rank], ws, bias, RES, r, out + at(t));
       }
-      const int c = (t << log_splits) + rank;
-      if (n8 < N)
-        store8<T>(sum, sx[c], ws, bias, res, out, (int64_t)(m0 + c) * N + n8, N - n8, wide);
+    } else {
+      int t = warp - 2;
+      float r[4], next[4] = {};
+      auto load = [&](int t) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (n_first + 32 * j < N) next[j] = ep_f(res[at(t) + 32 * j]);
+      };
+      if (RES && t < share(rank)) load(t);
+#pragma unroll 1
+      for (; t < share(rank); t += C::kEpiWarps) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) r[j] = next[j];
+        if (RES && t + C::kEpiWarps < share(rank)) load(t + C::kEpiWarps);
+        int sum[4] = {};
+#pragma unroll 1
+        for (int k = 0; k < splits; ++k)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            sum[j] += ld_shared(got + (k * run + t) * kColBytes + (lane + 32 * j) * 4);
+        const float s = sx[(t << log_splits) + rank];
+        T* o = out + at(t);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (n_first + 32 * j < N)
+            o[32 * j] = ep_t<T>(fmaf(static_cast<float>(sum[j]), s * ws[j], bias[j]) + r[j]);
+      }
     }
   }
   if (splits > 1) {
@@ -449,7 +491,7 @@ __device__ __forceinline__ void pair_tile(int t, int n_tiles, int m_tiles, int& 
   tn = g * kPairGroup + r - tm * width;
 }
 
-template <typename T>
+template <typename T, bool WIDE, bool RES>
 __global__ void __launch_bounds__(kPairThreads, 1)
     int8_pair_kernel(const __grid_constant__ CUtensorMap tm_w,
                      const __grid_constant__ CUtensorMap tm_x, const Epilogue e, int M, int N,
@@ -571,19 +613,20 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     const uint32_t mine = sb + kPairOffOut + (warp - 2) * (16 * 32 * 4);
     const T* res = static_cast<const T*>(e.residual);
     T* out = static_cast<T*>(e.out);
-    const bool wide = N % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0 &&
-                      (reinterpret_cast<uintptr_t>(res) & 15) == 0;
     int j = 0;
     for (int t = first; t < tiles; t += stride, ++j) {
       const int b = j & 1;
       int tn, tm;
       pair_tile(t, n_tiles, m_tiles, tn, tm);
-      const int n8 = tn * kPairRows + rank * 128 + 32 * q + 8 * (lane & 3), m0 = tm * kPairTokens;
+      // wide: eight adjacent outputs of two of sixteen tokens; else one output of all of them
+      const int n_warp = tn * kPairRows + rank * 128 + 32 * q, m0 = tm * kPairTokens;
+      const int n_first = n_warp + (WIDE ? 8 * (lane & 3) : lane);
       float ws[8], bias[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        ws[i] = n8 + i < N ? __ldg(e.weight_scale + n8 + i) : 0.f;
-        bias[i] = e.bias && n8 + i < N ? ep_f(static_cast<const T*>(e.bias)[n8 + i]) : 0.f;
+        const int n = n_first + i;
+        ws[i] = n < N ? __ldg(e.weight_scale + n) : 0.f;
+        bias[i] = e.bias && n < N ? ep_f(static_cast<const T*>(e.bias)[n]) : 0.f;
       }
       if (!mbar_wait(afull0 + 8 * b, (j >> 1) & 1, status)) {
         aborted = 1;
@@ -592,20 +635,46 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       tc_fence_after();
 #pragma unroll 1
       for (int c0 = half * (kPairTokens / 2); c0 < (half + 1) * (kPairTokens / 2) && m0 + c0 < M; c0 += 16) {
-        const int ma = m0 + c0 + (lane >> 2), mb = ma + 8;   // this thread's two tokens
-        const float sa = ma < M ? __ldg(e.scale + ma) : 0.f, sc = mb < M ? __ldg(e.scale + mb) : 0.f;
+        const int m = m0 + c0 + (lane & 15);
+        const float sx = m < M ? __ldg(e.scale + m) : 0.f;
         uint32_t v[16];
         tmem_ld16(tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)(b * kPairTokens + c0), v);
 #pragma unroll
         for (int i = 0; i < 16; ++i) st_shared(mine + (i * 32 + lane) * 4, v[i]);
         __syncwarp();
+        if constexpr (WIDE) {
+          Eight<T> r[2] = {};
+          const int a0 = lane >> 2;   // this thread's tokens of the sixteen: a0 and a0 + 8
+          const int64_t at = (int64_t)(m0 + c0 + a0) * N + n_first;
+          const bool in[2] = {n_first < N && m0 + c0 + a0 < M, n_first < N && m0 + c0 + a0 + 8 < M};
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          int sum[8];
-          ld_shared8(mine + ((i * 8 + (lane >> 2)) * 32 + 8 * (lane & 3)) * 4, sum);
-          const int m = i ? mb : ma;
-          if (n8 < N && m < M)
-            store8<T>(sum, i ? sc : sa, ws, bias, res, out, (int64_t)m * N + n8, N - n8, wide);
+          for (int i = 0; i < 2; ++i)
+            if (RES && in[i]) r[i].load(res + at + (int64_t)(8 * i) * N);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            int sum[8];
+            ld_shared8(mine + ((a0 + 8 * i) * 32 + 8 * (lane & 3)) * 4, sum);
+            const float s = __shfl_sync(0xffffffffu, sx, a0 + 8 * i);
+            if (in[i])
+              store8<T>(sum, s, ws, bias, RES, r[i], out + at + (int64_t)(8 * i) * N);
+          }
+        } else {
+#pragma unroll 1
+          for (int a0 = 0; a0 < 16; a0 += 8) {
+            const int64_t at = (int64_t)(m0 + c0 + a0) * N + n_first;
+            float r[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              r[i] = RES && n_first < N && m0 + c0 + a0 + i < M ? ep_f(res[at + (int64_t)i * N])
+                                                                : 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float s = __shfl_sync(0xffffffffu, sx, a0 + i);
+              const float sum = static_cast<float>(ld_shared(mine + ((a0 + i) * 32 + lane) * 4));
+              if (n_first < N && m0 + c0 + a0 + i < M)
+                out[at + (int64_t)i * N] = ep_t<T>(fmaf(sum, s * ws[0], bias[0]) + r[i]);
+            }
+          }
         }
         __syncwarp();   // read before the next tokens' sums are written
       }
@@ -682,10 +751,10 @@ int launch(const void* kern, int grid, int threads, int smem, int cluster, cudaS
   return launch_status("rw4 int8_linear launch");
 }
 
-template <int BN, typename T>
+template <int BN, typename T, bool WIDE, bool RES>
 int launch_split(const Problem& p) {
   using C = SplitCfg<BN>;
-  const void* kern = reinterpret_cast<const void*>(int8_split_kernel<BN, T>);
+  const void* kern = reinterpret_cast<const void*>(int8_split_kernel<BN, T, WIDE, RES>);
   static std::atomic<uint64_t> done{0};
   int st = set_smem(kern, C::kSmem, done);
   CUtensorMap w, x;
@@ -712,9 +781,9 @@ int launch_split(const Problem& p) {
                 args);
 }
 
-template <typename T>
+template <typename T, bool WIDE, bool RES>
 int launch_pair(const Problem& p) {
-  const void* kern = reinterpret_cast<const void*>(int8_pair_kernel<T>);
+  const void* kern = reinterpret_cast<const void*>(int8_pair_kernel<T, WIDE, RES>);
   static std::atomic<uint64_t> done{0};
   int st = set_smem(kern, kPairSmem, done);
   CUtensorMap w, x;
@@ -737,14 +806,25 @@ int launch_pair(const Problem& p) {
 //                     tiles: 13.4 against 17.0 for pairs), of 64 where even that leaves most SMs idle
 //                     (128 x 2048 x 2048, 16 tiles of 128: 6.1 against 7.6), else CTA pairs
 //                     (512 x 4096 x 6144, 192 tiles: 17.3 against 24.2 in two waves)
+template <typename T, bool WIDE, bool RES>
+int run_tiles(const Problem& p, int32_t path) {
+  const int64_t rows = (p.N + BMW - 1) / BMW, tiles128 = rows * ((p.M + 127) / 128);
+  if (path == 2 || (path == 0 && p.M > 64 && tiles128 > sm_count()))
+    return launch_pair<T, WIDE, RES>(p);
+  if (p.M <= 16) return launch_split<16, T, WIDE, RES>(p);
+  if (p.M <= 32) return launch_split<32, T, WIDE, RES>(p);
+  if (p.M <= 64 || tiles128 <= 32) return launch_split<64, T, WIDE, RES>(p);
+  return launch_split<128, T, WIDE, RES>(p);
+}
+
+// (the epilogue's forms are compiled apart: code that a launch does not run still cost a one-token
+// call half a microsecond of instruction fetches)
 template <typename T>
 int run(const Problem& p, int32_t path) {
-  const int64_t rows = (p.N + BMW - 1) / BMW, tiles128 = rows * ((p.M + 127) / 128);
-  if (path == 2 || (path == 0 && p.M > 64 && tiles128 > sm_count())) return launch_pair<T>(p);
-  if (p.M <= 16) return launch_split<16, T>(p);
-  if (p.M <= 32) return launch_split<32, T>(p);
-  if (p.M <= 64 || tiles128 <= 32) return launch_split<64, T>(p);
-  return launch_split<128, T>(p);
+  const bool wide = wide_rows(p.e, p.N), res = p.e.residual != nullptr;
+  if (wide)
+    return res ? run_tiles<T, true, true>(p, path) : run_tiles<T, true, false>(p, path);
+  return res ? run_tiles<T, false, true>(p, path) : run_tiles<T, false, false>(p, path);
 }
 
 }  // namespace
