@@ -208,6 +208,11 @@ struct SplitCfg {
   static_assert((kSmem + 1024) * kCtasPerSm <= 228 * 1024, "shared memory budget");
 };
 
+// k-blocks of the weight that a CTA prefetches into L2 before its turn (norm, products and quantizer
+// of a layer of width 8192 in one graph, one token: 151.8 us a layer without, 149.2 with 3, 151.8 with
+// 10, 157.6 with 20)
+constexpr int kPrefetch = 3;
+
 template <int BN, typename T, bool WIDE, bool RES>
 __global__ void __launch_bounds__(SplitCfg<BN>::kThreads)
     int8_split_kernel(const __grid_constant__ CUtensorMap tm_w,
@@ -255,6 +260,9 @@ __global__ void __launch_bounds__(SplitCfg<BN>::kThreads)
   if (warp == 0 && lane == 0) {
     prefetch_tensormap(&tm_w);
     prefetch_tensormap(&tm_x);
+    // the weight's first tiles into L2 while the kernel before this one runs (nothing is read that
+    // it could still write: L2 holds what is written)
+    for (int kb = kb0; kb < min(kb1, kb0 + kPrefetch); ++kb) tma_prefetch_2d(&tm_w, kb * BK, n0);
   }
   tc_fence_before();
   __syncthreads();

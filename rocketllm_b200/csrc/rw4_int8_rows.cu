@@ -610,7 +610,8 @@ int run_rows(const RowArgs& a, cudaStream_t stream) {
                                              threads_for((nvec + parts - 1) / parts, 1), stream);
   // With a CTA or less on every SM threads hide latency, beyond it registers do (norm with residual
   // of 4096 values: 150 rows 2.3 us with one vector a thread, 2.4 with two; 600 rows 6.2 and 5.5).
-  if (nvec <= kMaxThreads && (a.M <= sm_count() || nvec <= kMaxThreads / 2))
+  if (nvec <= kMaxThreads && (a.M <= sm_count() || nvec <= 3 * kMaxThreads / 8 ||
+                              (nvec <= kMaxThreads / 2 && a.M <= 8 * sm_count())))
     return launch_rows<T, MODE, 1, kBlock>(a, a.M, 1, threads_for(nvec, 1), stream);
   if (nvec <= 2 * kMaxThreads)
     return launch_rows<T, MODE, 2, kBlock>(a, a.M, 1, threads_for(nvec, 2), stream);

@@ -90,6 +90,77 @@ def test_rmsnorm(cuda, m, k, residual, dtype):
     check_rows(codes, scale, y, e=2.0 ** -19)
 
 
+# enough rows for every multiprocessor to take several in turn: whole 16-byte rows, odd ones, rows
+# in pieces over a cluster
+MANY = [(2500, 4096), (5100, 1032), (640, 14336), (310, 28672), (5100, 1037), (1900, 4099),
+        (640, 14335), (310, 20001), (170, 33001), (90, 65539), (90, 131056), (1900, 4100)]
+
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("m,k", MANY)
+def test_many_rows(cuda, m, k, dtype):
+    """Each operator over many rows, some of them zero, NaN or infinite, the first and last among
+    the ordinary ones; the residual stream in place."""
+    x = randn(m + k, m, k, dtype=dtype)
+    x[3], x[m // 2, k - 1], x[m - 2, 0] = 0, float("nan"), float("inf")
+    odd = torch.zeros(m, dtype=torch.bool, device="cuda")
+    odd[m // 2] = odd[m - 2] = True
+
+    def check(codes, scale, y, e):
+        assert scale[odd].isnan().all() and codes[odd].abs().max() == 0
+        check_rows(codes[~odd], scale[~odd], y[~odd], e)
+
+    check(*kernels.int8_quantize(x), x.double(), 0.0)
+    gu = randn(m + k + 1, m, 2 * k, dtype=dtype)
+    gate = gu[:, :k].double()
+    codes, scale = kernels.int8_quantize(gu[:, k:], gate=gu[:, :k])
+    check_rows(codes, scale, gate * torch.sigmoid(gate) * gu[:, k:].double(), 2.0 ** -19)
+    w = randn(k, k, dtype=dtype)
+    hd = x.double()
+    y = hd * torch.rsqrt(hd.square().mean(-1, keepdim=True) + 1e-5) * w.double()
+    check(*kernels.int8_rmsnorm(x, w, 1e-5), y, 2.0 ** -19)
+    r = gu[:, :k].contiguous()
+    h = (x.double() + r.double()).to(dtype)
+    codes, scale, got = kernels.int8_rmsnorm(x, w, 1e-5, residual=r, hidden=r)
+    assert got is r and torch.equal(got[~odd], h[~odd])
+    hd = h.double()
+    y = hd * torch.rsqrt(hd.square().mean(-1, keepdim=True) + 1e-5) * w.double()
+    check(codes, scale, y, 2.0 ** -19)
+    torch.cuda.synchronize()
+    assert kernels.device_status() == 0
+
+
+@pytest.mark.parametrize("m,k,ox,os,oc", [(1900, 4096, 1, 0, 0), (1900, 4096, 0, 3, 0),
+                                          (1900, 4096, 0, 0, 5), (1900, 4099, 2, 7, 1),
+                                          (90, 40000, 3, 5, 7)])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_many_rows_of_every_alignment(cuda, m, k, ox, os, oc, dtype):
+    """Strided inputs that start anywhere, codes and hidden rows that start anywhere; the bytes
+    around the outputs stay as they were."""
+    x = randn(1, m, k + 11, dtype=dtype)[:, ox:ox + k]
+    second = randn(2, m, k + 8, dtype=dtype)[:, os:os + k]
+    w = randn(3, k + 7, dtype=dtype)[oc:oc + k]
+    flat = torch.full((m * k + 64,), 77, dtype=torch.int8, device="cuda")
+    codes = flat[16 + oc:16 + oc + m * k].view(m, k)
+    hflat = torch.full((m * k + 64,), 77, dtype=dtype, device="cuda")
+    hidden = hflat[16 + os:16 + os + m * k].view(m, k)
+    out = (codes, torch.empty(m, device="cuda"))
+    kernels.int8_quantize(x, out=out)
+    check_rows(*out, x)
+    kernels.int8_quantize(x, gate=second, out=out)
+    g = second.double()
+    check_rows(*out, g * torch.sigmoid(g) * x.double(), e=2.0 ** -19)
+    kernels.int8_rmsnorm(x, w, 1e-5, residual=second, out=out, hidden=hidden)
+    assert torch.equal(hidden, (x.double() + second.double()).to(dtype))
+    hd = hidden.double()
+    check_rows(*out, hd * torch.rsqrt(hd.square().mean(-1, keepdim=True) + 1e-5) * w.double(),
+               e=2.0 ** -19)
+    for f, o in ((flat, oc), (hflat, os)):
+        assert (f[:16 + o] == 77).all() and (f[16 + o + m * k:] == 77).all()
+    torch.cuda.synchronize()
+    assert kernels.device_status() == 0
+
+
 def test_ties_round_to_even(cuda):
     """max |y| = 127 makes the factor exactly 1: halves are ties."""
     y = torch.tensor([[127.0, 0.5, 1.5, 2.5, -0.5, -1.5, -2.5, 126.5]], device="cuda")
