@@ -489,21 +489,41 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
                : "memory");
 }
 
-// Tile t of a grid of n_tiles x m_tiles: groups of kPairGroup weight tiles, tokens in the middle,
-// so that the tiles in flight form a near-square block whose operands L2 holds.
-__device__ __forceinline__ void pair_tile(int t, int n_tiles, int m_tiles, int& tn, int& tm) {
-  const int per = kPairGroup * m_tiles;
-  const int g = t / per, r = t - g * per;
-  const int width = min(kPairGroup, n_tiles - g * kPairGroup);
-  tm = r / width;
-  tn = g * kPairGroup + r - tm * width;
+// The tiles of a call: a grid of n_tiles x m_tiles, and how its last wave is cut.
+struct PairGrid {
+  int n_tiles, m_tiles;
+  int full;       // tiles that are taken whole, whole waves of them
+  int cut;        // each tile after them is taken as 1 << cut strips of 256 >> cut tokens
+  int items;      // tiles and strips
+};
+
+struct PairItem {
+  int n0, m0, width;   // first weight row, first token, tokens
+};
+
+// Item t.  Tiles come in groups of kPairGroup weight tiles, tokens in the middle, so that the tiles in
+// flight form a near-square block whose operands L2 holds.
+__device__ __forceinline__ PairItem pair_item(int t, const PairGrid& g) {
+  int strip = 0, width = kPairTokens;
+  if (t >= g.full) {
+    const int u = t - g.full;
+    strip = u & ((1 << g.cut) - 1);
+    t = g.full + (u >> g.cut);
+    width = kPairTokens >> g.cut;
+  }
+  const int per = kPairGroup * g.m_tiles;
+  const int group = t / per, r = t - group * per;
+  const int side = min(kPairGroup, g.n_tiles - group * kPairGroup);
+  const int tm = r / side, tn = group * kPairGroup + r - tm * side;
+  return {tn * kPairRows, tm * kPairTokens + strip * width, width};
 }
 
 template <typename T, bool WIDE, bool RES>
 __global__ void __launch_bounds__(kPairThreads, 1)
     int8_pair_kernel(const __grid_constant__ CUtensorMap tm_w,
-                     const __grid_constant__ CUtensorMap tm_x, const Epilogue e, int M, int N,
-                     int nkb, int n_tiles, int m_tiles, unsigned int* status) {
+                     const __grid_constant__ CUtensorMap tm_x,
+                     const __grid_constant__ CUtensorMap tm_strip, const Epilogue e, int M, int N,
+                     int nkb, const PairGrid g, unsigned int* status) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
@@ -516,7 +536,6 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + kPairOffTmem);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
-  const int tiles = n_tiles * m_tiles;
   const int first = blockIdx.x >> 1, stride = gridDim.x >> 1;
 
   if (threadIdx.x == 0) {
@@ -541,6 +560,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   if (warp == 0 && lane == 0) {
     prefetch_tensormap(&tm_w);
     prefetch_tensormap(&tm_x);
+    prefetch_tensormap(&tm_strip);
   }
   tc_fence_before();
   __syncthreads();
@@ -558,10 +578,12 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       // leader's arrival, and neither starts a stage before the commit of the MMAs that read it.)
       int i = 0;
       bool ok = true;
-      for (int t = first; t < tiles && ok; t += stride) {
-        int tn, tm;
-        pair_tile(t, n_tiles, m_tiles, tn, tm);
-        const int n0 = tn * kPairRows + rank * 128, m0 = tm * kPairTokens + rank * (kPairTokens / 2);
+      for (int t = first; t < g.items && ok; t += stride) {
+        const PairItem it = pair_item(t, g);
+        if (it.m0 >= M) continue;   // a strip past the last token (in every role)
+        const int n0 = it.n0 + rank * 128, m0 = it.m0 + rank * (it.width / 2);
+        const CUtensorMap* mx = t < g.full ? &tm_x : &tm_strip;
+        const uint32_t bytes = 2 * kWBytes + it.width * BK;   // of both CTAs
         for (int kb = 0; kb < nkb; ++kb, ++i) {
           const int s = i % kPairStages;
           if (!mbar_wait(empty0 + 8 * s, ((i / kPairStages) & 1) ^ 1, status)) {
@@ -571,9 +593,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           }
           const uint32_t bar = map_rank(full0 + 8 * s, 0);
           const uint32_t dst = sb + s * kPairStageBytes;
-          if (rank == 0) mbar_arrive_expect_tx(full0 + 8 * s, 2 * kPairStageBytes);
+          if (rank == 0) mbar_arrive_expect_tx(full0 + 8 * s, bytes);
           tma_load_2d_pair(dst, &tm_w, kb * BK, n0, bar);
-          tma_load_2d_pair(dst + kWBytes, &tm_x, kb * BK, m0, bar);
+          tma_load_2d_pair(dst + kWBytes, mx, kb * BK, m0, bar);
         }
       }
       if (!ok) {
@@ -586,7 +608,10 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     if (rank == 0 && lane == 0) {
       int i = 0, j = 0;
       bool ok = true;
-      for (int t = first; t < tiles && ok; t += stride, ++j) {
+      for (int t = first; t < g.items && ok; t += stride) {
+        const PairItem it = pair_item(t, g);
+        if (it.m0 >= M) continue;
+        const uint32_t idesc = idesc_i8(kPairRows, it.width);
         const int b = j & 1;
         if (!mbar_wait(aempty0 + 8 * b, ((j >> 1) & 1) ^ 1, status)) {
           aborted = 1;
@@ -606,10 +631,11 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 #pragma unroll
           for (int kk = 0; kk < BK / 32; ++kk)
             umma_i8_pair(tmem + b * kPairTokens, da + (uint64_t)(2 * kk), db + (uint64_t)(2 * kk),
-                         idesc_i8(kPairRows, kPairTokens), (kb > 0 || kk > 0) ? 1u : 0u);
+                         idesc, (kb > 0 || kk > 0) ? 1u : 0u);
           umma_commit_pair(empty0 + 8 * s);
         }
         umma_commit_pair(afull0 + 8 * b);
+        ++j;
       }
     }
   } else {
@@ -622,12 +648,12 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     const T* res = static_cast<const T*>(e.residual);
     T* out = static_cast<T*>(e.out);
     int j = 0;
-    for (int t = first; t < tiles; t += stride, ++j) {
+    for (int t = first; t < g.items; t += stride) {
+      const PairItem it = pair_item(t, g);
+      if (it.m0 >= M) continue;
       const int b = j & 1;
-      int tn, tm;
-      pair_tile(t, n_tiles, m_tiles, tn, tm);
       // wide: eight adjacent outputs of two of sixteen tokens; else one output of all of them
-      const int n_warp = tn * kPairRows + rank * 128 + 32 * q, m0 = tm * kPairTokens;
+      const int n_warp = it.n0 + rank * 128 + 32 * q, m0 = it.m0;
       const int n_first = n_warp + (WIDE ? 8 * (lane & 3) : lane);
       float ws[8], bias[8];
 #pragma unroll
@@ -642,7 +668,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       }
       tc_fence_after();
 #pragma unroll 1
-      for (int c0 = half * (kPairTokens / 2); c0 < (half + 1) * (kPairTokens / 2) && m0 + c0 < M; c0 += 16) {
+      for (int c0 = half * (it.width / 2); c0 < (half + 1) * (it.width / 2) && m0 + c0 < M; c0 += 16) {
         const int m = m0 + c0 + (lane & 15);
         const float sx = m < M ? __ldg(e.scale + m) : 0.f;
         uint32_t v[16];
@@ -689,6 +715,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(leader_empty + 8 * b);
+      ++j;
     }
   }
   __syncwarp();
@@ -794,18 +821,26 @@ int launch_pair(const Problem& p) {
   const void* kern = reinterpret_cast<const void*>(int8_pair_kernel<T, WIDE, RES>);
   static std::atomic<uint64_t> done{0};
   int st = set_smem(kern, kPairSmem, done);
-  CUtensorMap w, x;
-  if (st == RW4_OK) st = maps(p, kPairTokens / 2, &w, &x);
-  if (st != RW4_OK) return st;
   int M = (int)p.M, N = (int)p.N, nkb = (int)((p.K + BK - 1) / BK);
-  int n_tiles = (N + kPairRows - 1) / kPairRows, m_tiles = (M + kPairTokens - 1) / kPairTokens;
-  const int64_t tiles = (int64_t)n_tiles * m_tiles;
-  const int64_t pairs = sm_count() / 2;
+  PairGrid g;
+  g.n_tiles = (N + kPairRows - 1) / kPairRows;
+  g.m_tiles = (M + kPairTokens - 1) / kPairTokens;
+  // The tiles that do not fill a last wave are cut into strips of 128 or 64 tokens, as long as those
+  // fit in it (1500 x 4096 x 4096, 96 tiles for 74 pairs: 27.3 us whole, 25.2 cut; 700 x 8192 x 8192,
+  // 96 tiles: 45.4 and 43.2; narrower strips only wait for their operands).
+  const int tiles = g.n_tiles * g.m_tiles, pairs = sm_count() / 2, rest = tiles % pairs;
+  g.full = tiles - rest;
+  for (g.cut = 0; rest && g.cut < 2 && (rest << (g.cut + 1)) <= pairs;) ++g.cut;
+  g.items = g.full + (rest << g.cut);
+  CUtensorMap w, x, strip;
+  if (st == RW4_OK) st = maps(p, kPairTokens / 2, &w, &x);
+  if (st == RW4_OK) st = maps(p, (kPairTokens >> g.cut) / 2, &w, &strip);
+  if (st != RW4_OK) return st;
   Epilogue e = p.e;
   unsigned int* status = p.status;
-  void* args[] = {&w, &x, &e, &M, &N, &nkb, &n_tiles, &m_tiles, &status};
-  return launch(kern, 2 * (int)(tiles < pairs ? tiles : pairs), kPairThreads, kPairSmem, 2,
-                p.stream, args);
+  void* args[] = {&w, &x, &strip, &e, &M, &N, &nkb, &g, &status};
+  return launch(kern, 2 * (g.items < pairs ? g.items : pairs), kPairThreads, kPairSmem, 2, p.stream,
+                args);
 }
 
 // Which tiles (times of 148 SMs, in us):

@@ -352,7 +352,9 @@ def test_linear_epilogues(cuda, m, k, n, bias, residual, dtype):
 
 
 @pytest.mark.parametrize("m,k,n", [(1, 4096, 6144), (16, 14336, 4096), (333, 2048, 5632),
-                                   (2048, 4096, 1024), (1024, 8192, 8192), (4099, 1024, 4096)])
+                                   (2048, 4096, 1024), (1024, 8192, 8192), (4099, 1024, 4096),
+                                   (1500, 512, 4096), (2100, 256, 5000), (530, 384, 20000),
+                                   (1111, 640, 9999), (700, 512, 8200)])
 def test_linear_at_model_sizes(cuda, m, k, n):
     q, qs, w, ws, b, r = operands(k, m, k, n, residual=True)
     y = kernels.int8_linear(q, qs, w, ws, residual=r)
