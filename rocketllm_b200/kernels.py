@@ -258,7 +258,8 @@ def int8_quantize(x, gate=None, out=None):
     Float32, bfloat16 or float16; rows may be strided (halves of a concatenated projection).  In
     fp32, ``scale = max|y| / 127`` and ``codes = rint(y * (127 / max|y|))``; a row of zeros (or with
     ``max|y| < 2**-119``) has scale 0, a row that holds a NaN or an infinity scale NaN, both codes
-    0.  ``out``: ``(codes, scale)`` to write instead of new tensors.
+    0.  ``out``: ``(codes, scale)`` to write instead of new tensors.  Forward only, as the other
+    8-bit calls: results carry no gradient.
     """
     if _native is not None and out is None:
         done = _native.int8_quantize(x, gate)

@@ -16,6 +16,8 @@ Tolerances, derived (u = 2^-24, half a step of fp32):
   then one rounding to the output's type, eps / 2 of the value (below the smallest normal number:
   of that number).
 """
+import threading
+
 import pytest
 import torch
 
@@ -517,6 +519,40 @@ def test_weights_written_just_before_they_are_read(cuda):
             want = y
         elif it % 2 == 0:
             assert torch.equal(y, want)
+
+
+def test_calls_at_once(cuda):
+    """Threads on streams of their own: products of both kinds, the 4-bit product's tensor-core
+    kernel and the row kernels at the same time give what they give alone."""
+    from rocketllm_b200.synthetic import make_activation, make_weight
+    pair, split = operands(1, 600, 512, 9000), operands(2, 40, 2048, 1024)
+    rows = randn(3, 2500, 4096)
+    packed = make_weight(4096, 1024, device=cuda, seed=4)
+    x4 = make_activation(200, 1024, device=cuda, seed=5)
+
+    def calls():
+        return [kernels.int8_linear(*pair[:4]), kernels.int8_linear(*split[:4]),
+                *kernels.int8_quantize(rows), kernels.linear(x4, *packed)]
+
+    want = calls()
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(25):
+                got = calls()[::-1 if i % 2 else 1]
+                stream.synchronize()
+                bad.extend(k for k, (a, b) in enumerate(zip(got, want[::-1 if i % 2 else 1]))
+                           if not torch.equal(a, b))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad and kernels.device_status() == 0
 
 
 def test_native_and_ctypes_calls_agree(cuda, monkeypatch):
