@@ -403,12 +403,13 @@ constexpr int kRingNV = 4;
 constexpr int kRingStages = 2;       // at most
 constexpr int kRingThreads = 1024;   // at most (64 registers a thread)
 
+// L2 drops these lines first: the inputs are not read again, the codes written beside them are.
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes,
-                                          uint32_t bar) {
+                                          uint32_t bar, uint64_t policy) {
   asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::
-          "r"(dst),
-      "l"(src), "r"(bytes), "r"(bar)
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], "
+      "%2, [%3], %4;" ::"r"(dst),
+      "l"(src), "r"(bytes), "r"(bar), "l"(policy)
       : "memory");
 }
 
@@ -439,20 +440,21 @@ __global__ void __launch_bounds__(kRingThreads, 1)
   }
   __syncthreads();
   pdl_enter();
+  const uint64_t once = policy_evict_first();
   auto issue = [&](int64_t j) {   // thread 0
     const int64_t row = blockIdx.x + j * gridDim.x;
     const int s = static_cast<int>(j % stages);
     const uint32_t dst = smem_addr(ring) + s * stage_bytes, bar = bar0 + 8 * s;
     mbar_arrive_expect_tx(bar, stage_bytes);
-    bulk_load(dst, static_cast<const T*>(a.x) + row * a.x_ld, row_bytes, bar);
+    bulk_load(dst, static_cast<const T*>(a.x) + row * a.x_ld, row_bytes, bar, once);
     if (kTwo)
       bulk_load(dst + row_bytes, static_cast<const T*>(a.second) + row * a.second_ld, row_bytes,
-                bar);
+                bar, once);
   };
   if (threadIdx.x == 0) {
     if (MODE >= kNorm) {
       mbar_arrive_expect_tx(wbar, row_bytes);
-      bulk_load(smem_addr(smem), a.weight, row_bytes, wbar);
+      bulk_load(smem_addr(smem), a.weight, row_bytes, wbar, policy_evict_last());
     }
     for (int64_t j = 0; j < stages && j < mine; ++j) issue(j);
   }
