@@ -150,3 +150,16 @@ def test_int4_kv_cache_and_batches(checkpoint):
     out = model.generate(ids, attention_mask=mask, max_new_tokens=4, do_sample=False,
                          pad_token_id=0)
     assert out.shape == (2, 24)
+
+
+@pytest.mark.parametrize("batch", [1, 3])
+def test_graphed_decode(checkpoint, batch):
+    """The CUDA-graphed decode step over RW8 layers: the same tokens as the same step launched
+    eagerly, in a graph that stays alive beside a second one."""
+    from rocketllm_b200.decode import GraphedDecoder
+    model = AutoModel.from_pretrained(checkpoint).model
+    ids = prompt(12, batch)
+    eager = GraphedDecoder(model, batch, 64, use_graph=False).generate(ids, 16)
+    decoders = [GraphedDecoder(model, batch, 64) for _ in range(2)]
+    got = [d.generate(ids, 16) for d in decoders]
+    assert torch.equal(got[0], eager) and torch.equal(got[1], eager)
