@@ -166,6 +166,15 @@ __device__ __forceinline__ uint4 load_cached(const void* p) {
   return v;
 }
 
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+
 // Eight values of a row as their inputs' type holds them (16 or 32 bytes of registers).
 template <typename T>
 struct Held {
@@ -187,6 +196,24 @@ struct Held {
 #pragma unroll
     for (int j = 0; j < kQuads; ++j) u[j] = reinterpret_cast<const uint4*>(t)[j];
   }
+  // the eight values that start `shift` bytes into kQuads + 1 granules
+  __device__ __forceinline__ void take(uint32_t (&w)[4 * kQuads + 4], int shift) {
+    if (shift & 8) {
+#pragma unroll
+      for (int j = 0; j < 4 * kQuads + 2; ++j) w[j] = w[j + 2];
+    }
+    if (shift & 4) {
+#pragma unroll
+      for (int j = 0; j < 4 * kQuads + 1; ++j) w[j] = w[j + 1];
+    }
+    if (sizeof(T) == 2 && (shift & 2)) {
+#pragma unroll
+      for (int j = 0; j < 4 * kQuads; ++j) w[j] = __byte_perm(w[j], w[j + 1], 0x5432);
+    }
+#pragma unroll
+    for (int j = 0; j < kQuads; ++j)
+      u[j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+  }
   // Values i .. i+7 of a row of K (0 outside it).  `shift`: bytes past a 16-byte boundary at
   // which every vector of this row starts; kKeep: the row is read again (kept in L1).
   template <bool kKeep>
@@ -206,21 +233,7 @@ struct Held {
         const uint4 q = load_cached(g + j);
         w[4 * j] = q.x, w[4 * j + 1] = q.y, w[4 * j + 2] = q.z, w[4 * j + 3] = q.w;
       }
-      if (shift & 8) {
-#pragma unroll
-        for (int j = 0; j < 4 * kQuads + 2; ++j) w[j] = w[j + 2];
-      }
-      if (shift & 4) {
-#pragma unroll
-        for (int j = 0; j < 4 * kQuads + 1; ++j) w[j] = w[j + 1];
-      }
-      if (sizeof(T) == 2 && (shift & 2)) {
-#pragma unroll
-        for (int j = 0; j < 4 * kQuads; ++j) w[j] = __byte_perm(w[j], w[j + 1], 0x5432);
-      }
-#pragma unroll
-      for (int j = 0; j < kQuads; ++j)
-        u[j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+      take(w, shift);
     } else {
       float v[8];
 #pragma unroll
@@ -231,6 +244,36 @@ struct Held {
   __device__ __forceinline__ void load_shared(const T* p) {
 #pragma unroll
     for (int j = 0; j < kQuads; ++j) u[j] = reinterpret_cast<const uint4*>(p)[j];
+  }
+  // from shared memory, `shift` bytes past a 16-byte boundary
+  __device__ __forceinline__ void load_shared_at(uint32_t addr, int shift) {
+    if (shift == 0) {
+#pragma unroll
+      for (int j = 0; j < kQuads; ++j) u[j] = lds128(addr + 16 * j);
+    } else {
+      uint32_t w[4 * kQuads + 4];
+#pragma unroll
+      for (int j = 0; j <= kQuads; ++j) {
+        const uint4 q = lds128(addr - shift + 16 * j);
+        w[4 * j] = q.x, w[4 * j + 1] = q.y, w[4 * j + 2] = q.z, w[4 * j + 3] = q.w;
+      }
+      take(w, shift);
+    }
+  }
+  // value by value
+  __device__ __forceinline__ void load_values(const T* row, int i, int K) {
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) v[j] = i + j >= 0 && i + j < K ? to_f(row[i + j]) : 0.f;
+    set(v);
+  }
+  // keep the values of positions i .. i+7 that lie in a row of K
+  __device__ __forceinline__ void clip(int i, int K) {
+    float v[8];
+    get(v);
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) v[j] = i + j >= 0 && i + j < K ? v[j] : 0.f;
+    set(v);
   }
   // `aligned`: every vector of this row starts on 16 bytes
   __device__ __forceinline__ void store(T* row, int i, int K, bool aligned) const {
@@ -505,6 +548,170 @@ __global__ void __launch_bounds__(kRingThreads, 1)
   }
 }
 
+// The quantizer's ring for rows of any length, alignment and stride, and for rows longer than a CTA
+// holds: the parts CTAs of a cluster take a piece of every row each, of vp vectors, and exchange
+// their sums once a row.  A piece is copied as the 16-byte granules that it touches, and its vectors
+// are shifted out of them.  Those granules lie inside the tensor except at its two ends: in its first
+// and last row a granule that reaches past the first or last value is not copied, and the vectors
+// that need it are read value by value.  (2877 x 11660: quantize 29.1 us with a CTA a row, 25.0 here,
+// swiglu 59.6 and 41.6; 496 x 21731 fp32: 18.5 and 13.5, 56 and 30.  A norm, whose weight has to be
+// shifted too, lost: 57.8 and 72.8.)
+struct Piece {
+  const uint8_t* from;   // first granule copied
+  uint32_t bytes;        // of the granules copied
+  uint32_t skip;         // where they go: bytes past the first granule touched (0 or 16)
+  bool no_lo, no_hi;     // the first / last granule touched is not copied
+};
+
+template <typename T>
+__device__ __forceinline__ Piece piece_of(const T* base, int64_t ld, int64_t M, int K, int64_t row,
+                                          int e0, int e1) {
+  const uintptr_t lo = reinterpret_cast<uintptr_t>(base);
+  const uintptr_t hi = lo + ((M - 1) * ld + K) * sizeof(T);
+  const uintptr_t a = lo + (row * ld + e0) * sizeof(T), e = lo + (row * ld + e1) * sizeof(T);
+  uintptr_t g0 = a & ~uintptr_t(15), g1 = (e + 15) & ~uintptr_t(15);
+  Piece p;
+  p.no_lo = g0 < lo;
+  p.no_hi = g1 > hi;
+  p.skip = p.no_lo ? 16 : 0;
+  if (p.no_lo) g0 += 16;
+  if (p.no_hi) g1 -= 16;
+  p.from = reinterpret_cast<const uint8_t*>(g0);
+  p.bytes = g1 > g0 ? static_cast<uint32_t>(g1 - g0) : 0;
+  return p;
+}
+
+constexpr int kRingPad = 64;   // shared memory before and after a piece that vectors may read
+
+template <typename T, int MODE, bool SPLIT>
+__global__ void __launch_bounds__(kRingThreads, 1)
+    ring_any_kernel(const RowArgs a, int parts, int vp, int piece_bytes, int stages,
+                    unsigned int* status) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ uint64_t bars[kRingStages];
+  __shared__ RowSums part[2][32];
+  __shared__ RowSums join[2];
+  __shared__ volatile int aborted;
+  static_assert(MODE == kPlain || MODE == kGated);
+  constexpr bool kTwo = MODE == kGated;
+  constexpr int NV = kRingNV, es = sizeof(T);
+  const int K = a.K;
+  const int rank = SPLIT ? blockIdx.x % parts : 0;
+  const int64_t first = SPLIT ? blockIdx.x / parts : blockIdx.x;
+  const int64_t stride = SPLIT ? gridDim.x / parts : gridDim.x;
+  const int64_t mine = (a.M - first + stride - 1) / stride;
+  const uint32_t stage_bytes = kTwo ? 2 * piece_bytes : piece_bytes;
+  const uint32_t ring = smem_addr(smem), bar0 = smem_addr(bars);
+  const T* x = static_cast<const T*>(a.x);
+  const T* second = static_cast<const T*>(a.second);
+  const int piece0 = rank * vp * kVec, piece1 = piece0 + vp * kVec;   // this CTA's, before the lead
+  // the last bits of an address p + (row * ld + i) * size: products need no more than theirs
+  auto low = [](const void* p, int64_t row, int64_t ld, int i, int size, int mask) {
+    return (static_cast<int>(reinterpret_cast<uintptr_t>(p)) +
+            (static_cast<int>(row) * static_cast<int>(ld) + i) * size) & mask;
+  };
+  if (threadIdx.x == 0) {
+    aborted = 0;
+    for (int s = 0; s < kRingStages; ++s) mbar_init(bar0 + 8 * s, 1);
+    fence_barrier_init();
+  }
+  __syncthreads();
+  pdl_enter();
+  const uint64_t once = policy_evict_first();
+  auto issue = [&](int64_t j) {   // thread 0
+    const int64_t row = first + j * stride;
+    const int s = static_cast<int>(j % stages), lead = low(a.codes, row, K, 0, 1, 7);
+    const int e0 = max(0, piece0 - lead), e1 = min(K, piece1 - lead);
+    const uint32_t dst = ring + s * stage_bytes + kRingPad, bar = bar0 + 8 * s;
+    const Piece p = piece_of(x, a.x_ld, a.M, K, row, e0, e1);
+    Piece q = {};
+    if (kTwo) q = piece_of(second, a.second_ld, a.M, K, row, e0, e1);
+    mbar_arrive_expect_tx(bar, p.bytes + q.bytes);
+    if (p.bytes) bulk_load(dst + p.skip, p.from, p.bytes, bar, once);
+    if (q.bytes) bulk_load(dst + piece_bytes + q.skip, q.from, q.bytes, bar, once);
+  };
+  if (threadIdx.x == 0)
+    for (int64_t j = 0; j < stages && j < mine; ++j) issue(j);
+  const int tbase = piece0 + static_cast<int>(threadIdx.x) * kVec, step = blockDim.x * kVec;
+  int s = 0;
+  uint32_t phase = 0;
+  for (int64_t j = 0; j < mine; ++j) {
+    const int64_t row = first + j * stride;
+    const int lead = low(a.codes, row, K, 0, 1, 7);
+    const int e0 = max(0, piece0 - lead), e1 = min(K, piece1 - lead), end = piece1 - lead;
+    const int base = tbase - lead;
+    // shared addresses of value 0 of the row, and what every vector is past a boundary
+    const uint32_t at = ring + s * stage_bytes + kRingPad - e0 * es;
+    const uint32_t xz = at + low(x, row, a.x_ld, e0, es, 15);
+    const uint32_t sz = at + piece_bytes + (kTwo ? low(second, row, a.second_ld, e0, es, 15) : 0);
+    const int x_shift = (xz + base * es) & 15, s_shift = (sz + base * es) & 15;
+    Piece p = {}, q = {};
+    if (row == 0 || row == a.M - 1) {
+      p = piece_of(x, a.x_ld, a.M, K, row, e0, e1);
+      if (kTwo) q = piece_of(second, a.second_ld, a.M, K, row, e0, e1);
+    }
+    // (after a wait that ran out the rest of the loop only keeps the barriers in step)
+    if (!aborted && !mbar_wait(bar0 + 8 * s, phase, status)) aborted = 1;
+    float y[NV][kVec];
+    RowSums sums = {0.f, 0.f};
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      const int i = base + n * step;
+      if (i >= K || i >= end) continue;
+      Held<T> h, g;
+      h.load_shared_at(xz + i * es, x_shift);
+      if constexpr (kTwo) g.load_shared_at(sz + i * es, s_shift);
+      if (i < e0 + kVec || i + 2 * kVec > e1) {   // the piece's ends
+        if ((p.no_lo && i < e0 + kVec) || (p.no_hi && i + 2 * kVec > e1)) {
+          h.load_values(x + row * a.x_ld, i, K);
+        } else {
+          h.clip(i, K);
+        }
+        if constexpr (kTwo) {
+          if ((q.no_lo && i < e0 + kVec) || (q.no_hi && i + 2 * kVec > e1)) {
+            g.load_values(second + row * a.second_ld, i, K);
+          } else {
+            g.clip(i, K);
+          }
+        }
+      }
+      combine<T, MODE>(h, g, g, y[n], sums.ss);
+      sums.top = top_of(y[n], sums.top);
+    }
+    // the stage's values are in registers: order these reads before the copy that refills it
+    fence_proxy_async_smem();
+    sums = block_sums<MODE>(sums, part[j & 1]);
+    if (threadIdx.x == 0 && j + stages < mine && !aborted) issue(j + stages);
+    if constexpr (SPLIT) {
+      // (two slots in turn, as for the warps' sums)
+      if (threadIdx.x == 0) join[j & 1] = sums;
+      cg::this_cluster().sync();
+      const int lane = threadIdx.x & 31;
+      sums = warp_sums<MODE>(lane < parts ? *cg::this_cluster().map_shared_rank(&join[j & 1], lane)
+                                          : RowSums{0.f, 0.f});
+    }
+    const RowScale r8 = row_scale<MODE>(sums, K, a.eps);
+    if (!aborted) {
+      if (threadIdx.x == 0 && rank == 0) a.scale[row] = r8.scale;
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        const int i = base + n * step;
+        if (i < K && i < end) store_codes(a.codes + row * K, i, K, y[n], r8);
+      }
+    }
+    if (++s == stages) {
+      s = 0;
+      phase ^= 1;
+    }
+  }
+  if (aborted) {
+    // leave the copies in flight time to land before the shared memory goes
+    const unsigned long long t0 = globaltimer();
+    while (globaltimer() - t0 < 2000000ull) __nanosleep(1000);
+  }
+  if constexpr (SPLIT) cg::this_cluster().sync();   // the others have read this CTA's last sums
+}
+
 template <typename T, int MODE, int NV, int KIND>
 int launch_rows(const RowArgs& a, int64_t blocks, int parts, int threads, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
@@ -525,75 +732,104 @@ int launch_rows(const RowArgs& a, int64_t blocks, int parts, int threads, cudaSt
   return rw4::launch_status("rw4 int8 rows launch");
 }
 
-// Whether the ring takes the call, and its shape: whole 16-byte rows, enough of them for every CTA.
+struct RingShape {
+  int parts, vp, threads, piece, stages, grid, smem;
+};
+
+// How a ring takes rows of nvec vectors; false where it does not: short rows (a warp each), or
+// fewer than two rows for every CTA (then a CTA per row is faster: 1001 x 5632, norm 6.1 us against
+// 7.9).  pad: bytes around a piece in shared memory (0: whole rows, as they are).
 template <typename T, int MODE>
-bool ring_shape(const RowArgs& a, int& threads, int& stages, int& grid, int& smem) {
-  constexpr int es = sizeof(T);
-  auto whole = [](const void* p, int64_t ld) { return aligned(p, 16) && ld * es % 16 == 0; };
-  const int nvec = a.K / kVec;
-  if (a.K % kVec || nvec <= 128 || nvec > kRingNV * kRingThreads || !whole(a.x, a.x_ld) ||
-      !whole(a.second, a.second_ld) || !aligned(a.weight, 16) || !aligned(a.hidden, 16) ||
-      !aligned(a.codes, 8))
-    return false;
-  threads = ((nvec + kRingNV - 1) / kRingNV + 31) / 32 * 32;
-  const int row = a.K * es, stage = MODE == kGated || MODE == kNormRes ? 2 * row : row;
-  const int fixed = MODE >= kNorm ? row : 0;
-  int per_sm = kRingThreads / threads;   // 64 registers a thread
-  if (per_sm > 16) per_sm = 16;
-  auto fits = [&](int n) { return 227 * 1024 / (fixed + n * stage + 2048); };
-  // two stages as long as two CTAs an SM hold them (or the one that its threads allow): below that
-  // a second CTA hides more than a second stage (swiglu 2048 x 14336: 31.5 us with two CTAs of one
-  // stage, 34.0 with one of two; norm with residual 8192 x 8192: 73 us with two CTAs of two
-  // stages, 83 with four of one)
-  stages = fits(2) >= (per_sm < 2 ? per_sm : 2) ? 2 : 1;
-  const int f = fits(stages);
-  if (f < 1) return false;
-  if (per_sm > f) per_sm = f;
-  smem = fixed + stages * stage;
-  const int64_t ctas = static_cast<int64_t>(sm_count()) * per_sm;
-  // below two rows a CTA a CTA per row is faster (1001 x 5632: norm 7.9 us against 6.1)
-  if (a.M < 2 * ctas) return false;
-  grid = static_cast<int>(ctas);
-  return true;
+bool ring_shape(const RowArgs& a, int nvec, int pad, RingShape& r) {
+  if (nvec <= 128) return false;
+  for (r.parts = 1; r.parts <= (pad ? 8 : 1); r.parts *= 2) {
+    r.vp = (nvec + r.parts - 1) / r.parts;
+    r.threads = ((r.vp + kRingNV - 1) / kRingNV + 31) / 32 * 32;
+    if (r.threads > kRingThreads) continue;
+    const int values = pad ? r.vp * kVec + kVec : a.K;
+    r.piece = (values * static_cast<int>(sizeof(T)) + 15) / 16 * 16 + 2 * pad;
+    const int stage = MODE == kGated || MODE == kNormRes ? 2 * r.piece : r.piece;
+    const int fixed = MODE >= kNorm ? r.piece : 0;
+    int per_sm = kRingThreads / r.threads;   // 64 registers a thread
+    if (per_sm > 16) per_sm = 16;
+    auto fits = [&](int n) { return 227 * 1024 / (fixed + n * stage + 2048); };
+    // two stages as long as two CTAs an SM hold them (or the one that its threads allow): below
+    // that a second CTA hides more than a second stage (swiglu 2048 x 14336: 31.5 us with two CTAs
+    // of one stage, 34.0 with one of two; norm with residual 8192 x 8192: 73 us with two CTAs of two
+    // stages, 83 with four of one)
+    r.stages = fits(2) >= (per_sm < 2 ? per_sm : 2) ? 2 : 1;
+    const int f = fits(r.stages);
+    if (f < 1) continue;
+    if (per_sm > f) per_sm = f;
+    r.smem = fixed + r.stages * stage;
+    r.grid = sm_count() * per_sm / r.parts * r.parts;
+    return a.M >= 2 * static_cast<int64_t>(r.grid) / r.parts;
+  }
+  return false;
 }
 
-template <typename T, int MODE>
-int launch_ring(const RowArgs& a, int threads, int stages, int grid, int smem,
-                cudaStream_t stream) {
-  static std::atomic<uint64_t> done{0};
+// Whole 16-byte rows at 16-byte addresses.
+template <typename T>
+bool whole_rows(const RowArgs& a) {
+  auto whole = [](const void* p, int64_t ld) {
+    return aligned(p, 16) && ld * static_cast<int>(sizeof(T)) % 16 == 0;
+  };
+  return a.K % kVec == 0 && whole(a.x, a.x_ld) && whole(a.second, a.second_ld) &&
+         aligned(a.weight, 16) && aligned(a.hidden, 16) && aligned(a.codes, kVec);
+}
+
+template <typename... KArgs, typename... Args>
+int launch_ring(void (*kern)(KArgs...), std::atomic<uint64_t>& done, const RingShape& r,
+                cudaStream_t stream, Args... args) {
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev >= 64 || !((done.load() >> dev) & 1)) {
-    if (cudaFuncSetAttribute(ring_kernel<T, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             225 * 1024) != cudaSuccess)
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 225 * 1024) !=
+        cudaSuccess)
       return fail(RW4_ECUDA, "int8 rows: cannot set the kernel's shared memory size");
     if (dev < 64) done.fetch_or(1ull << dev);
   }
-  unsigned int* status = device_status_ptr();
-  if (!status) return fail(RW4_ECUDA, "int8 rows: device status word unavailable");
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
+  cfg.gridDim = dim3(r.grid);
+  cfg.blockDim = dim3(r.threads);
+  cfg.dynamicSmemBytes = r.smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = r.parts;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t err = cudaLaunchKernelEx(&cfg, ring_kernel<T, MODE>, a, stages, status);
+  cfg.numAttrs = r.parts > 1 ? 2 : 1;
+  const cudaError_t err = cudaLaunchKernelEx(&cfg, kern, args...);
   if (err != cudaSuccess) return cuda_status(err, "rw4 int8 rows launch");
   return launch_status("rw4 int8 rows launch");
 }
 
 template <typename T, int MODE>
 int run_rows(const RowArgs& a, cudaStream_t stream) {
-  int threads, stages, grid, smem;
-  if (ring_shape<T, MODE>(a, threads, stages, grid, smem))
-    return launch_ring<T, MODE>(a, threads, stages, grid, smem, stream);
   // a row's vectors, with one more where it can start inside one
-  const bool whole = a.K % kVec == 0 && rw4::aligned(a.codes, kVec);
+  const bool whole = a.K % kVec == 0 && aligned(a.codes, kVec);
   const int nvec = whole ? a.K / kVec : (a.K + 2 * (kVec - 1)) / kVec;
+  unsigned int* status = device_status_ptr();
+  if (!status) return fail(RW4_ECUDA, "int8 rows: device status word unavailable");
+  RingShape r;
+  static std::atomic<uint64_t> done[3];
+  if (whole_rows<T>(a) && ring_shape<T, MODE>(a, nvec, 0, r))
+    return launch_ring(ring_kernel<T, MODE>, done[0], r, stream, a, r.stages, status);
+  if constexpr (MODE == kPlain || MODE == kGated) {
+    // (long rows of two aligned inputs: 512 x 53248 44.4 us with a cluster a row, 48.3 in this ring)
+    if (nvec > 1024 && (MODE == kPlain || !whole_rows<T>(a)) &&
+        ring_shape<T, MODE>(a, nvec, kRingPad, r)) {
+      if (r.parts == 1)
+        return launch_ring(ring_any_kernel<T, MODE, false>, done[1], r, stream, a, 1, r.vp, r.piece,
+                           r.stages, status);
+      return launch_ring(ring_any_kernel<T, MODE, true>, done[2], r, stream, a, r.parts, r.vp,
+                         r.piece, r.stages, status);
+    }
+  }
   if (nvec <= 128) {   // one warp a row, four rows a CTA
     const int64_t blocks = (a.M + kWarpThreads / 32 - 1) / (kWarpThreads / 32);
     if (nvec <= 32) return launch_rows<T, MODE, 1, kWarp>(a, blocks, 1, kWarpThreads, stream);
