@@ -552,7 +552,7 @@ __global__ void __launch_bounds__(kRingThreads, 1)
 // holds: the parts CTAs of a cluster take a piece of every row each, of vp vectors, and exchange
 // their sums once a row.  A piece is copied as the 16-byte granules that it touches, and its vectors
 // are shifted out of them.  Those granules lie inside the tensor except at its two ends: in its first
-// and last row a granule that reaches past the first or last value is not copied, and the vectors
+// and last row (any row, where rows overlap) a granule that reaches past the first or last value is not copied, and the vectors
 // that need it are read value by value.  (2877 x 11660: quantize 29.1 us with a CTA a row, 25.0 here,
 // swiglu 59.6 and 41.6; 496 x 21731 fp32: 18.5 and 13.5, 56 and 30.  A norm, whose weight has to be
 // shifted too, lost: 57.8 and 72.8.)
@@ -607,9 +607,12 @@ __global__ void __launch_bounds__(kRingThreads, 1)
   const int piece0 = rank * vp * kVec, piece1 = piece0 + vp * kVec;   // this CTA's, before the lead
   // the last bits of an address p + (row * ld + i) * size: products need no more than theirs
   auto low = [](const void* p, int64_t row, int64_t ld, int i, int size, int mask) {
-    return (static_cast<int>(reinterpret_cast<uintptr_t>(p)) +
-            (static_cast<int>(row) * static_cast<int>(ld) + i) * size) & mask;
+    return static_cast<int>((static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) +
+                             (static_cast<uint32_t>(row) * static_cast<uint32_t>(ld) +
+                              static_cast<uint32_t>(i)) * static_cast<uint32_t>(size)) & mask);
   };
+  // rows that overlap can all lie at an end of the tensor
+  const bool overlap = a.x_ld < K || (kTwo && a.second_ld < K);
   if (threadIdx.x == 0) {
     aborted = 0;
     for (int s = 0; s < kRingStages; ++s) mbar_init(bar0 + 8 * s, 1);
@@ -646,7 +649,7 @@ __global__ void __launch_bounds__(kRingThreads, 1)
     const uint32_t sz = at + piece_bytes + (kTwo ? low(second, row, a.second_ld, e0, es, 15) : 0);
     const int x_shift = (xz + base * es) & 15, s_shift = (sz + base * es) & 15;
     Piece p = {}, q = {};
-    if (row == 0 || row == a.M - 1) {
+    if (row == 0 || row == a.M - 1 || overlap) {
       p = piece_of(x, a.x_ld, a.M, K, row, e0, e1);
       if (kTwo) q = piece_of(second, a.second_ld, a.M, K, row, e0, e1);
     }

@@ -163,6 +163,26 @@ def test_many_rows_of_every_alignment(cuda, m, k, ox, os, oc, dtype):
     assert kernels.device_status() == 0
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("stride", [0, 1, 8])
+def test_many_overlapping_rows(cuda, stride, dtype):
+    """Broadcast rows and rows a few values apart, from an unaligned start, enough of them for every
+    path of the row kernels."""
+    for m, k in ((700, 20003), (700, 33001), (2000, 4099), (2000, 4096)):
+        flat = randn(k + stride, 3 + k + stride * m, dtype=dtype)
+        x = flat[3:].as_strided((m, k), (stride, 1), 3)
+        want = kernels.int8_quantize(x.contiguous())
+        assert all(torch.equal(a, b) for a, b in zip(kernels.int8_quantize(x), want))
+        want = kernels.int8_quantize(x.contiguous(), gate=x.contiguous())
+        assert all(torch.equal(a, b) for a, b in zip(kernels.int8_quantize(x, gate=x), want))
+        w = randn(1, k, dtype=dtype)
+        want = kernels.int8_rmsnorm(x.contiguous(), w, 1e-5, residual=x.contiguous())
+        got = kernels.int8_rmsnorm(x, w, 1e-5, residual=x)
+        assert torch.equal(got[2], want[2]) and torch.equal(got[0], want[0])
+        # (another path may sum the squares in another order)
+        assert ((got[1] - want[1]).abs() <= 2.0 ** -19 * want[1]).all()
+
+
 def test_ties_round_to_even(cuda):
     """max |y| = 127 makes the factor exactly 1: halves are ties."""
     y = torch.tensor([[127.0, 0.5, 1.5, 2.5, -0.5, -1.5, -2.5, 126.5]], device="cuda")
