@@ -784,6 +784,8 @@ bool whole_rows(const RowArgs& a) {
 template <typename... KArgs, typename... Args>
 int launch_ring(void (*kern)(KArgs...), std::atomic<uint64_t>& done, const RingShape& r,
                 cudaStream_t stream, Args... args) {
+  unsigned int* status = device_status_ptr();
+  if (!status) return fail(RW4_ECUDA, "int8 rows: device status word unavailable");
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev >= 64 || !((done.load() >> dev) & 1)) {
@@ -806,7 +808,7 @@ int launch_ring(void (*kern)(KArgs...), std::atomic<uint64_t>& done, const RingS
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = r.parts > 1 ? 2 : 1;
-  const cudaError_t err = cudaLaunchKernelEx(&cfg, kern, args...);
+  const cudaError_t err = cudaLaunchKernelEx(&cfg, kern, args..., status);
   if (err != cudaSuccess) return cuda_status(err, "rw4 int8 rows launch");
   return launch_status("rw4 int8 rows launch");
 }
@@ -816,21 +818,19 @@ int run_rows(const RowArgs& a, cudaStream_t stream) {
   // a row's vectors, with one more where it can start inside one
   const bool whole = a.K % kVec == 0 && aligned(a.codes, kVec);
   const int nvec = whole ? a.K / kVec : (a.K + 2 * (kVec - 1)) / kVec;
-  unsigned int* status = device_status_ptr();
-  if (!status) return fail(RW4_ECUDA, "int8 rows: device status word unavailable");
   RingShape r;
   static std::atomic<uint64_t> done[3];
   if (whole_rows<T>(a) && ring_shape<T, MODE>(a, nvec, 0, r))
-    return launch_ring(ring_kernel<T, MODE>, done[0], r, stream, a, r.stages, status);
+    return launch_ring(ring_kernel<T, MODE>, done[0], r, stream, a, r.stages);
   if constexpr (MODE == kPlain || MODE == kGated) {
     // (long rows of two aligned inputs: 512 x 53248 44.4 us with a cluster a row, 48.3 in this ring)
     if (nvec > 1024 && (MODE == kPlain || !whole_rows<T>(a)) &&
         ring_shape<T, MODE>(a, nvec, kRingPad, r)) {
       if (r.parts == 1)
         return launch_ring(ring_any_kernel<T, MODE, false>, done[1], r, stream, a, 1, r.vp, r.piece,
-                           r.stages, status);
+                           r.stages);
       return launch_ring(ring_any_kernel<T, MODE, true>, done[2], r, stream, a, r.parts, r.vp,
-                         r.piece, r.stages, status);
+                         r.piece, r.stages);
     }
   }
   if (nvec <= 128) {   // one warp a row, four rows a CTA
