@@ -2,11 +2,12 @@
 //
 // A decode-sized call of these operators takes 1.5 to 8 us on the GPU; checking its arguments,
 // allocating its results and marshalling a dozen values through ctypes takes 9 to 19 us in Python
-// and 3.5 to 5 us here (the launch itself 2.1).  Each function takes the plain case -- CUDA tensors of the documented types
-// and shapes, all on the current device, results to be allocated -- makes the same C-ABI call
-// (include/rw4.h) on the current stream and returns the results.  For anything else it returns
-// None and has done nothing: the Python entry point then goes on with its own checks, which make
-// the errors, the compact copies, the writes into given outputs and the calls on other devices.
+// and 3.5 to 5 us here (of which the launch itself is 2.1).  Each function takes the plain case --
+// CUDA tensors of the documented types and shapes, all on the current device, results to be
+// allocated -- makes the same C-ABI call (include/rw4.h) on the current stream and returns the
+// results.  For anything else it returns None and has launched nothing: the Python entry point then
+// goes on with its own checks, which make the errors, the compact copies, the writes into given
+// outputs and the calls on other devices.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 

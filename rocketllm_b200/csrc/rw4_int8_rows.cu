@@ -551,11 +551,11 @@ __global__ void __launch_bounds__(kRingThreads, 1)
 // The quantizer's ring for rows of any length, alignment and stride, and for rows longer than a CTA
 // holds: the parts CTAs of a cluster take a piece of every row each, of vp vectors, and exchange
 // their sums once a row.  A piece is copied as the 16-byte granules that it touches, and its vectors
-// are shifted out of them.  Those granules lie inside the tensor except at its two ends: in its first
-// and last row (any row, where rows overlap) a granule that reaches past the first or last value is not copied, and the vectors
-// that need it are read value by value.  (2877 x 11660: quantize 29.1 us with a CTA a row, 25.0 here,
-// swiglu 59.6 and 41.6; 496 x 21731 fp32: 18.5 and 13.5, 56 and 30.  A norm, whose weight has to be
-// shifted too, lost: 57.8 and 72.8.)
+// are shifted out of them.  Those granules lie inside the tensor except at its two ends: in its
+// first and last row (any row, where rows overlap) a granule that reaches past the first or last
+// value is not copied, and the vectors that need it are read value by value.  (2877 x 11660:
+// quantize 29.1 us with a CTA a row, 25.0 here, swiglu 59.6 and 41.6; 496 x 21731 fp32: 18.5 and
+// 13.5, 56 and 30.  A norm, whose weight has to be shifted too, lost: 57.8 and 72.8.)
 struct Piece {
   const uint8_t* from;   // first granule copied
   uint32_t bytes;        // of the granules copied
