@@ -16,7 +16,7 @@ Tolerances, derived (u = 2^-24, half a step of fp32):
   then one rounding to the output's type, eps / 2 of the value (below the smallest normal number:
   of that number).
 """
-import threading
+from concurrent.futures import ThreadPoolExecutor
 
 import pytest
 import torch
@@ -567,12 +567,53 @@ def test_calls_at_once(cuda):
                 bad.extend(k for k, (a, b) in enumerate(zip(got, want[::-1 if i % 2 else 1]))
                            if not torch.equal(a, b))
 
-    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
-    for t in threads:
-        t.start()
-    for t in threads:
-        t.join()
+    with ThreadPoolExecutor(4) as pool:
+        for done in [pool.submit(work, i) for i in range(4)]:
+            done.result()
     assert not bad and kernels.device_status() == 0
+
+
+def _linear_calls():
+    q, qs, w, ws = operands(1, 40, 2048, 1024)[:4]
+    q2, qs2, w2, ws2 = operands(2, 600, 512, 9000)[:4]
+    return [lambda out=None: kernels.int8_linear(q, qs, w, ws, out=out),
+            lambda out=None: kernels.int8_linear(q2, qs2, w2, ws2, out=out)]
+
+
+def _packed_calls():
+    from rocketllm_b200.synthetic import make_activation, make_weight
+    packed = make_weight(4096, 1024, device="cuda", seed=4)
+    few, many = (make_activation(m, 1024, device="cuda", seed=5) for m in (1, 200))
+    return [lambda out=None: kernels.linear(few, *packed, out=out),
+            lambda out=None: kernels.linear(many, *packed, out=out)]
+
+
+@pytest.mark.parametrize("make", [_linear_calls, _packed_calls])
+@pytest.mark.parametrize("captured", [False, True])
+def test_first_call_of_a_thread(cuda, make, captured):
+    """A product can be the first CUDA call that a thread makes: its results in memory that the
+    allocator holds already, or given, on a stream that is captured."""
+    for call in make():
+        want, stream = call(), torch.cuda.Stream()
+        out = torch.zeros_like(want) if captured else None
+        with torch.cuda.stream(stream):
+            call()                 # leaves its memory with the stream
+        torch.cuda.synchronize()
+
+        def work():
+            torch.cuda.set_stream(stream)
+            return call(out)
+
+        with ThreadPoolExecutor(1) as pool:
+            if captured:
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph, stream=stream, capture_error_mode="relaxed"):
+                    got = pool.submit(work).result()
+                graph.replay()
+            else:
+                got = pool.submit(work).result()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
 
 
 def test_native_and_ctypes_calls_agree(cuda, monkeypatch):
