@@ -455,6 +455,15 @@ constexpr int kPairThreads = 32 * (2 + kPairEpiWarps);
 constexpr uint32_t kPairTmemCols = 2 * kPairTokens;              // two accumulators
 constexpr int kPairGroup = 8;                   // weight tiles that run side by side
 static_assert(kPairSmem <= 227 * 1024, "shared memory budget");
+// A CTA whose TMEM allocation waits must not wait for a cluster that waits in turn for this one's.
+// This kernel takes all columns, but its shared memory leaves an SM no room for a CTA of another
+// cluster kernel that allocates any; the CTAs of the split kernel that fit on an SM leave each other
+// their columns.
+static_assert(kPairSmem + SplitCfg<16>::kSmem > 228 * 1024 &&
+              kPairSmem + SplitCfg<32>::kSmem > 228 * 1024 &&
+              kPairSmem + SplitCfg<64>::kSmem > 228 * 1024 &&
+              kPairSmem + SplitCfg<128>::kSmem > 228 * 1024, "no pair CTA beside a split CTA");
+static_assert(2 * (SplitCfg<64>::kTmemCols + SplitCfg<128>::kTmemCols) <= 512, "TMEM columns");
 
 // Plain load into this CTA's shared memory whose bytes complete on a barrier of the pair's leader.
 __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, int x, int y,
