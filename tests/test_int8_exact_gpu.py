@@ -1,0 +1,38 @@
+"""What the 8-bit operators promise at the ends of their ranges and at ties, against formulas.
+
+Tolerances, derived (u = 2^-24, half a step of fp32; the row checks are those of test_int8_gpu.py):
+
+* codes of a tensor are rint(y * (127 / a)) with both operations rounded to fp32: the same bits as
+  the same two operations of IEEE arithmetic anywhere, and the scale those of a / 127.
+"""
+import numpy as np
+import pytest
+import torch
+
+from rocketllm_b200 import kernels
+from test_int8_gpu import BF, F16, F32, randn
+
+pytestmark = pytest.mark.gpu
+
+
+# a warp, a CTA or a cluster a row, one and several vectors a thread; the rings, with whole rows, any
+# rows, and rows in pieces over a cluster
+SHAPES = [(1, 8), (9, 509), (3, 1000), (2, 4096), (20, 14336), (2, 16385), (2, 53248), (2500, 4096),
+          (640, 14336), (310, 28672), (640, 14335), (170, 33001)]
+
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("m,k", SHAPES)
+def test_codes_are_the_rounded_product(cuda, m, k, dtype):
+    """16-bit rows hold many values at an exact half of a code, each row's factor 127 / a rounded:
+    the product is rounded to fp32 before it is rounded to a code."""
+    x = randn(m + k, m, k, dtype=dtype)
+    x[0, 0], x[0, k - 1] = 2.03125, 1.015625      # 63.5 of 127: to 64
+    x[0].clamp_(-2.03125, 2.03125)
+    codes, scale = kernels.int8_quantize(x)
+    y = x.float().cpu().numpy()
+    a = np.abs(y).max(1, keepdims=True)
+    want = np.rint(y * (np.float32(127) / a))
+    assert np.array_equal(codes.cpu().numpy(), want)
+    assert np.array_equal(scale.cpu().numpy(), (a / np.float32(127))[:, 0])
+    assert codes[0, k - 1].item() == 64
