@@ -4,13 +4,17 @@ Tolerances, derived (u = 2^-24, half a step of fp32; the row checks are those of
 
 * codes of a tensor are rint(y * (127 / a)) with both operations rounded to fp32: the same bits as
   the same two operations of IEEE arithmetic anywhere, and the scale those of a / 127.
+* silu(g) * v for g down to -120: a = |g| log2(e) / 2 <= 86.6 is rounded (half a step: 2^-18; its
+  constant is off by 2^-26.2: 2^-19.7 here), which moves h = 2^-a by ln 2 of that and h^2 by twice as
+  much: 7 * 2^-20; the approximate exponential is off by 2^-22, twice, the reciprocal by 2^-23, five
+  roundings by u each.  e <= 8.1 * 2^-20 < 2^-16.
 """
 import numpy as np
 import pytest
 import torch
 
 from rocketllm_b200 import kernels
-from test_int8_gpu import BF, F16, F32, randn
+from test_int8_gpu import BF, F16, F32, check_rows, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -36,3 +40,24 @@ def test_codes_are_the_rounded_product(cuda, m, k, dtype):
     assert np.array_equal(codes.cpu().numpy(), want)
     assert np.array_equal(scale.cpu().numpy(), (a / np.float32(127))[:, 0])
     assert codes[0, k - 1].item() == 64
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("m,k", SHAPES)
+def test_gates_far_below_zero(cuda, m, k, dtype):
+    """Rows whose gates all lie where exp(g) is near the end of fp32 or past it, beside ordinary ones:
+    their products are far above the smallest scale."""
+    g = torch.Generator(device="cuda").manual_seed(m + k)
+    gate = -20 - 67 * torch.rand(m, k, generator=g, device="cuda")
+    gate[::3] = -87.5 - torch.rand(gate[::3].shape, generator=g, device="cuda")
+    gate[1::3] = torch.randn(gate[1::3].shape, generator=g, device="cuda") * 30
+    up = randn(k, m, k, dtype=F32) * 1e12
+    gate[0], up[0] = -88, 1e6
+    if m > 1:
+        gate[m - 1] = -92 - 28 * torch.rand(k, generator=g, device="cuda")
+        up[m - 1] = 1e36
+    gate, up = gate.to(dtype), up.to(dtype)
+    codes, scale = kernels.int8_quantize(up, gate=gate)
+    assert (codes[0] == -127).all()
+    gd = gate.double()
+    check_rows(codes, scale, gd * torch.sigmoid(gd) * up.double(), e=2.0 ** -16)
