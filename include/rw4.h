@@ -470,8 +470,8 @@ int rw4_int8_dequantize(const int8_t* codes, const float* scale, int64_t M, int6
                         int32_t out_dtype, void* stream);
 
 /* hidden = x + residual rounded to dtype (residual and hidden both null: hidden is x itself), and
- * codes, scale = quantized rows of hidden * rsqrt(mean(hidden^2) + eps) * weight, all in fp32
- * (stored as zeros where max |hidden * weight| is below 2^-119, too).
+ * codes, scale = quantized rows of hidden * rsqrt(mean(hidden^2) + eps) * weight, all in fp32 (for
+ * any finite hidden, also where its squares or its products with the weight leave fp32).
  * hidden may be residual or x itself (same address, contiguous rows). */
 int rw4_int8_rmsnorm(const void* x, int64_t x_stride, const void* residual,
                      int64_t residual_stride, const void* weight, int32_t dtype, int64_t M,

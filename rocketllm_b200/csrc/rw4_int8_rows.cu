@@ -10,9 +10,10 @@
 // normed row and the product to bf16 first, which costs accuracy and saves nothing here).
 //   - In a norm, rsqrt(..) is one factor r of the whole row: code = rint(h w * (127 / max |h w|)) and
 //     scale = r * max |h w| / 127, so the sum of squares and the maximum are taken in one pass and
-//     joined across the row in one exchange, and no value is multiplied by r.
-//   - A row whose scale would be subnormal (max |y|, or max |h w|, or a, below 2^-119) is stored as
-//     scale 0 and codes 0: below it 127 / a overflows fp32.
+//     joined across the row in one exchange, and no value is multiplied by r.  Rows whose squares or
+//     products leave fp32 that way, though y does not, are taken again with h scaled (scaled_norm).
+//   - A row whose scale would be subnormal (a below 2^-119) is stored as scale 0 and codes 0: below
+//     it 127 / a overflows fp32.
 //   - A row that holds a NaN or an infinity is stored as scale NaN and codes 0, so that what reads
 //     the row is NaN instead of a finite number.  The maximum is the NaN-propagating one.
 //   - Rounding to a code is the addition of 1.5 * 2^23 to the scaled value: the sum's low byte is the
@@ -303,14 +304,29 @@ struct RowScale {
   bool bad;
 };
 
-// A row's scale, and the factor to its codes.
+// What a norm's root is taken of.
+__device__ __forceinline__ float norm_mean(const RowSums& v, int K, float eps) {
+  return v.ss / static_cast<float>(K) + eps;
+}
+
+// A row's scale, and the factor to its codes.  `bad`: the row is stored as scale NaN and codes 0,
+// because it holds a NaN or an infinity or, in a norm, because its squares or its products h w are
+// not finite or so small that codes would be taken from subnormal numbers; scaled_norm then takes
+// it again.  (A mean from 2^-60 on keeps the factor below 2^30: products that vanish stand for values
+// below 2^-119.)
 template <int MODE>
 __device__ __forceinline__ RowScale row_scale(const RowSums& v, int K, float eps) {
-  const float a = MODE >= kNorm ? rsqrtf(v.ss / static_cast<float>(K) + eps) * v.top : v.top;
-  RowScale r = {0.f, 0.f, !(v.top < INFINITY) || !(a < INFINITY)};
+  float a = v.top;
+  RowScale r = {0.f, 0.f, false};
+  if constexpr (MODE >= kNorm) {
+    const float mean = norm_mean(v, K, eps);
+    a *= rsqrtf(mean);
+    r.bad = !(mean < INFINITY) || mean < 0x1p-60f || (v.top < kTiny && v.top > 0.f);
+  }
+  r.bad |= !(a < INFINITY);
   if (r.bad) {
     r.scale = __uint_as_float(0x7fc00000u);
-  } else if (v.top >= kTiny && a >= kTiny) {
+  } else if (a >= kTiny) {
     r.scale = __fdiv_rn(a, 127.f);
     r.inv = __fdiv_rn(127.f, v.top);
   }
@@ -325,6 +341,11 @@ __device__ __forceinline__ void round_pair(float a, float b, float inv, uint32_t
       " add.rn.f32x2 v, v, f;\n mov.b64 {%0, %1}, v;\n}\n"
       : "=r"(ca), "=r"(cb)
       : "f"(__fmul_rn(a, inv)), "f"(__fmul_rn(b, inv)), "f"(12582912.f));
+}
+
+// One code.
+__device__ __forceinline__ int8_t code_of(float y, const RowScale& r) {
+  return r.bad ? 0 : static_cast<int8_t>(__float_as_uint(__fadd_rn(__fmul_rn(y, r.inv), 12582912.f)));
 }
 
 // The codes of values i .. i+7 of a row of K (i on an 8-byte boundary of the codes).
@@ -392,6 +413,63 @@ __device__ __forceinline__ void combine(Held<T>& h, const Held<T>& second, const
 // who holds a row
 enum Kind { kWarp = 0, kBlock = 1, kCluster = 2 };
 
+// The sums of all that hold a row, once more (`part` and `join` may still be read for the last).
+template <int KIND>
+__device__ __forceinline__ RowSums row_sums_again(RowSums v, RowSums* part, RowSums* join) {
+  if constexpr (KIND == kWarp) return warp_sums<kNorm>(v);
+  if constexpr (KIND == kBlock) __syncthreads();
+  if constexpr (KIND == kCluster) cg::this_cluster().sync();
+  v = block_sums<kNorm>(v, part);
+  if constexpr (KIND == kCluster) {
+    if (threadIdx.x == 0) *join = v;
+    cg::this_cluster().sync();
+    const int lane = threadIdx.x & 31;
+    v = warp_sums<kNorm>(lane < static_cast<int>(cg::this_cluster().num_blocks())
+                             ? *cg::this_cluster().map_shared_rank(join, lane)
+                             : RowSums{0.f, 0.f});
+  }
+  return v;
+}
+
+// A norm's row, stored as a NaN one, by its definition, with h times a power of two that keeps its
+// squares inside fp32: y = (h f) rsqrt(mean (h f)^2 + eps f^2) w.  The row is read again (`h`: x, or
+// the hidden row, whose values each thread wrote itself) for the mean, the squares, the maximum and
+// the codes: such rows are rare, and the others' registers and time are not spent on them.  (It comes
+// after the first codes and scale: in their place it cost norm 1001 x 5632 6.7 us against 5.6, and
+// 515 x 2048 in fp32, 2.7 us without it, takes 3.0 either way.)
+// f = 2^84 for a mean below 2^-60 keeps 131056 squares under 2^125, 2^-84 from 2^60 on those of any
+// finite h.
+template <typename T, int KIND>
+__device__ __forceinline__ void scaled_norm(const T* h, const T* weight, int8_t* codes, float* scale,
+                                            int K, int base, int step, float eps, RowSums* part,
+                                            RowSums* join, bool first) {
+  auto sum_of = [&](float f) {
+    RowSums v = {0.f, 0.f};
+#pragma unroll 1
+    for (int i0 = base; i0 < K; i0 += step)
+#pragma unroll 1
+      for (int i = max(i0, 0); i < min(i0 + kVec, K); ++i)
+        v.ss = fmaf(to_f(h[i]) * f, to_f(h[i]) * f, v.ss);
+    return norm_mean(row_sums_again<KIND>(v, part, join), K, eps * f * f);
+  };
+  const float mean = sum_of(1.f);
+  const float f = mean < 0x1p-60f ? 0x1p84f : mean < 0x1p60f ? 1.f : 0x1p-84f;
+  const float r = rsqrtf(sum_of(f));
+  auto normed = [&](int i) { return to_f(h[i]) * f * r * to_f(weight[i]); };
+  RowSums v = {0.f, 0.f};
+#pragma unroll 1
+  for (int i0 = base; i0 < K; i0 += step)
+#pragma unroll 1
+    for (int i = max(i0, 0); i < min(i0 + kVec, K); ++i) v.top = top3(v.top, normed(i), 0.f);
+  const RowScale r8 = row_scale<kPlain>(row_sums_again<KIND>(v, part, join), K, 0.f);
+  if (r8.bad) return;
+  if (first) *scale = r8.scale;
+#pragma unroll 1
+  for (int i0 = base; i0 < K; i0 += step)
+#pragma unroll 1
+    for (int i = max(i0, 0); i < min(i0 + kVec, K); ++i) codes[i] = code_of(normed(i), r8);
+}
+
 template <typename T, int MODE, int NV, int KIND>
 __global__ void __launch_bounds__(KIND == kWarp ? kWarpThreads : kMaxThreads,
                                   KIND == kWarp ? 4 : sizeof(T) == 4 && NV == 4 ? 1 : 2)
@@ -455,11 +533,17 @@ __global__ void __launch_bounds__(KIND == kWarp ? kWarpThreads : kMaxThreads,
     sums = warp_sums<MODE>(lane < parts ? *cg::this_cluster().map_shared_rank(&join, lane)
                                         : RowSums{0.f, 0.f});
   }
+  const bool writes_scale =
+      rank == 0 && (KIND == kWarp ? threadIdx.x & 31 : threadIdx.x) == 0;
   const RowScale r8 = row_scale<MODE>(sums, K, a.eps);
-  if (rank == 0 && (KIND == kWarp ? threadIdx.x & 31 : threadIdx.x) == 0) a.scale[row] = r8.scale;
+  if (writes_scale) a.scale[row] = r8.scale;
 #pragma unroll
   for (int n = 0; n < NV; ++n)
     if (base + n * step < K) store_codes(codes, base + n * step, K, y[n], r8);
+  if constexpr (MODE >= kNorm)
+    if (r8.bad)   // (the same for all that hold the row)
+      scaled_norm<T, KIND>(MODE == kNormRes ? hidden : x, weight, codes, a.scale + row, K, base,
+                           step, a.eps, part, &join, writes_scale);
   if constexpr (KIND == kCluster) cg::this_cluster().sync();  // all have read the others' sums
 }
 
@@ -526,6 +610,7 @@ __global__ void __launch_bounds__(kRingThreads, 1)
   }
   if (MODE >= kNorm && !mbar_wait(wbar, 0, status)) aborted = 1;
   const int base = threadIdx.x * kVec, step = blockDim.x * kVec;
+  bool again = false;   // a norm's row is to be taken again (the same for the whole CTA)
   int s = 0;
   uint32_t phase = 0;
   for (int64_t j = 0; j < mine; ++j) {
@@ -553,6 +638,7 @@ __global__ void __launch_bounds__(kRingThreads, 1)
     sums = block_sums<MODE>(sums, part[j & 1]);
     if (threadIdx.x == 0 && j + stages < mine && !aborted) issue(j + stages);
     const RowScale r8 = row_scale<MODE>(sums, K, a.eps);
+    if (MODE >= kNorm) again |= r8.bad;
     if (!aborted) {
       if (threadIdx.x == 0) a.scale[row] = r8.scale;
 #pragma unroll
@@ -562,6 +648,17 @@ __global__ void __launch_bounds__(kRingThreads, 1)
     if (++s == stages) {
       s = 0;
       phase ^= 1;
+    }
+  }
+  if constexpr (MODE >= kNorm) {
+    if (again) {
+      __syncthreads();   // thread 0's scales, and a last word on `aborted`
+      for (int64_t row = blockIdx.x; row < a.M && !aborted; row += gridDim.x)
+        if (isnan(*static_cast<volatile float*>(a.scale + row)))
+          scaled_norm<T, kBlock>(MODE == kNormRes ? static_cast<const T*>(a.hidden) + row * K
+                                                  : static_cast<const T*>(a.x) + row * a.x_ld,
+                                 static_cast<const T*>(a.weight), a.codes + row * K, a.scale + row,
+                                 K, base, step, a.eps, part[0], nullptr, threadIdx.x == 0);
     }
   }
   if (aborted) {

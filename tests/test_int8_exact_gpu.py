@@ -61,3 +61,42 @@ def test_gates_far_below_zero(cuda, m, k, dtype):
     assert (codes[0] == -127).all()
     gd = gate.double()
     check_rows(codes, scale, gd * torch.sigmoid(gd) * up.double(), e=2.0 ** -16)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("eps", [0.0, 1e-5])
+@pytest.mark.parametrize("m,k", SHAPES)
+def test_norms_whose_squares_leave_fp32(cuda, m, k, eps, residual, dtype):
+    """Finite rows whose squares, or whose products with the weight, are above fp32's largest number
+    or below its smallest, among ordinary ones, a NaN and an infinite one."""
+    sizes = torch.tensor([1e25, 1.0, 1e37, 1e-15, 1e18, 1e-22, 1e-30, 1e-37], device="cuda")
+    x = (randn(m + k, m, k, dtype=F32) * sizes[torch.arange(m, device="cuda") % 8, None]).to(dtype)
+    odd = torch.zeros(m, dtype=torch.bool, device="cuda")
+    if m > 8:
+        x[5, k // 2], x[6, k - 1] = float("nan"), float("inf")
+        odd[5] = odd[6] = True
+    for big in (1.0, 1e20):
+        w = (randn(k, k, dtype=F32) * big).to(dtype)
+        h = x
+        if residual:
+            r = x / 2
+            want = (x.double() + r.double()).to(dtype)
+            codes, scale, h = kernels.int8_rmsnorm(x, w, eps, residual=r, hidden=r)
+            assert torch.equal(h[~odd], want[~odd]) and h is r
+        else:
+            codes, scale = kernels.int8_rmsnorm(x, w, eps)
+        assert scale[odd].isnan().all() and not codes[odd].any()
+        hd = h[~odd].double()
+        y = hd * torch.rsqrt(hd.square().mean(-1, keepdim=True) + eps) * w.double()
+        check_rows(codes[~odd], scale[~odd], y, e=2.0 ** -19)
+    # the largest finite rows, and a weight that is not finite
+    x[:] = torch.finfo(dtype).min
+    w = torch.ones(k, dtype=dtype, device="cuda")
+    codes, scale = kernels.int8_rmsnorm(x, w, eps)
+    assert (codes == -127).all() and ((scale * 127 - 1).abs() < 2.0 ** -19).all()
+    w[k // 2] = float("inf")
+    codes, scale = kernels.int8_rmsnorm(x, w, eps)
+    assert scale.isnan().all() and not codes.any()
+    torch.cuda.synchronize()
+    assert kernels.device_status() == 0
