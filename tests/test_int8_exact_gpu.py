@@ -8,13 +8,15 @@ Tolerances, derived (u = 2^-24, half a step of fp32; the row checks are those of
   constant is off by 2^-26.2: 2^-19.7 here), which moves h = 2^-a by ln 2 of that and h^2 by twice as
   much: 7 * 2^-20; the approximate exponential is off by 2^-22, twice, the reciprocal by 2^-23, five
   roundings by u each.  e <= 8.1 * 2^-20 < 2^-16.
+* a product of scales and a sum, as in test_int8_gpu.py, and half a step of fp32's subnormal numbers
+  (2^-150) more where it is one.
 """
 import numpy as np
 import pytest
 import torch
 
 from rocketllm_b200 import kernels
-from test_int8_gpu import BF, F16, F32, check_rows, randn
+from test_int8_gpu import BF, F16, F32, check_rows, operands, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -100,3 +102,38 @@ def test_norms_whose_squares_leave_fp32(cuda, m, k, eps, residual, dtype):
     assert scale.isnan().all() and not codes.any()
     torch.cuda.synchronize()
     assert kernels.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("path", [1, 2])
+@pytest.mark.parametrize("m,k,n", [(1, 1024, 300), (40, 4096, 512), (300, 512, 264)])
+def test_scales_whose_product_is_small(cuda, m, k, n, path, dtype):
+    """Scales whose product lies below 2^-126 beside results that do not, and scales far apart: no
+    bits are lost on the way."""
+    q, qs, w, ws, b, r = operands(m + k, m, k, n)
+    f = torch.finfo(dtype)
+
+    def check(y, q, ss, tt):
+        ref = q.double() @ w.double().t() * ss.double()[:, None] * tt.double()
+        err32 = 2.0 ** -22 * ref.abs() + 2.0 ** -150
+        bound = err32 + f.eps / 2 * (ref.abs() + err32).clamp_min(f.smallest_normal)
+        assert ((y.double() - ref).abs() <= bound).all()
+
+    for s, t in ((2.0 ** -100, 2.0 ** -40), (2.0 ** -40, 2.0 ** -100), (2.0 ** -70, 2.0 ** -70),
+                 (2.0 ** 110, 2.0 ** -120), (2.0 ** -120, 2.0 ** 90)):
+        for both in (False, True):      # every token, or every other
+            ss = qs.clone()
+            ss[::1 if both else 2] *= s
+            tt = ws * k * t
+            y = kernels.int8_linear(q, ss, w, tt, dtype=dtype, path=path)
+            check(y, q, ss, tt)
+    # (zero, huge and NaN scales keep to themselves)
+    ss, tt = qs.clone(), ws * 2.0 ** -60
+    ss[0], tt[n // 2] = 2.0 ** 120, 0
+    ss[m // 2] = 0
+    ss[m - 1] = float("nan")
+    y = kernels.int8_linear(q, ss, w, tt, dtype=dtype, path=path)
+    assert y[m - 1].isnan().all()
+    if m > 1:
+        check(y[:m - 1], q[:m - 1], ss[:m - 1], tt)
+        assert not y[m // 2].any() and not y[:m - 1, n // 2].any()
