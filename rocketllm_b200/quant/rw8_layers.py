@@ -50,9 +50,14 @@ def fuse_rw8_layers(model):
 
 
 def _norm(module, x, residual=None):
-    w = module.weight
-    return kernels.int8_rmsnorm(x, w if w.dtype == x.dtype else w.to(x.dtype),
-                                float(module.variance_epsilon), residual=residual)
+    w, eps = module.weight, float(module.variance_epsilon)
+    if w.dtype == x.dtype:
+        return kernels.int8_rmsnorm(x, w, eps, residual=residual)
+    # a weight of another type (fp32 norms in a 16-bit model) is not rounded to the stream's: the
+    # stream is rounded where int8_rmsnorm rounds it, the norm is taken in fp32
+    h = x if residual is None else x + residual
+    codes, scale = kernels.int8_rmsnorm(h.float(), w.float(), eps)
+    return (codes, scale) if residual is None else (codes, scale, h)
 
 
 def rw8_layer_forward(self, hidden_states, attention_mask=None, position_ids=None,
