@@ -112,7 +112,12 @@ class RW8Linear(nn.Module):
             codes, scale = kernels.int8_quantize(x)
         bias = self.bias
         if bias is not None and bias.dtype != x.dtype:
-            bias = bias.to(x.dtype)
+            # a bias of another type is not rounded to x's: the call in fp32, and the same one
+            # rounding at its end
+            y = kernels.int8_linear(codes, scale, self.weight, self.weight_scale,
+                                    bias=bias.float(), dtype=torch.float32,
+                                    residual=None if residual is None else residual.float())
+            return y.to(x.dtype)
         return kernels.int8_linear(codes, scale, self.weight, self.weight_scale, bias=bias,
                                    residual=residual, dtype=x.dtype)
 

@@ -4,8 +4,8 @@ from types import SimpleNamespace
 import pytest
 import torch
 
-from rocketllm_b200.quant import rw8_layers
-from test_int8_gpu import BF, F16, F32, check_rows, randn
+from rocketllm_b200.quant import Int8Rows, RW8Linear, rw8_layers
+from test_int8_gpu import BF, F16, F32, check_linear, check_rows, operands, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -24,3 +24,18 @@ def test_wider_norm_weights_are_not_rounded(cuda, dtype):
     codes, scale, h = rw8_layers._norm(norm, x, residual=r)
     assert h.dtype == dtype and torch.equal(h, (x.double() + r.double()).to(dtype))
     check_rows(codes, scale, normed(h), e=2.0 ** -19)
+
+
+@pytest.mark.parametrize("dtype", [BF, F16])
+def test_wider_biases_are_not_rounded(cuda, dtype):
+    """Rows in 16 bits beside a bias in 32: one rounding, of the whole sum."""
+    q, qs, wq, wsc, _, res = operands(4, 5, 512, 320, dtype, residual=True)
+    m = RW8Linear(512, 320, bias=True, device=cuda, dtype=F32)
+    m.weight.data, m.weight_scale.data = wq, wsc[:, None]
+    m.bias.data = randn(5, 320, dtype=F32) * 100
+    y = m(Int8Rows(q, qs, dtype))
+    assert y.dtype == dtype
+    check_linear(y, q, qs, wq, wsc, m.bias)
+    y = m(Int8Rows(q, qs, dtype), residual=res)
+    assert y.dtype == dtype
+    check_linear(y, q, qs, wq, wsc, m.bias, res)
