@@ -14,8 +14,15 @@ keeps the attention module and computes
 
 Parameters are read at every call, so a streamed layer (whose parameters are views into the engine's
 slots) takes the same path.
+
+The norms and the MLP are not called as modules here, and the projections that read 8-bit rows get
+:class:`Int8Rows`.  So a layer in which something waits for those calls -- a forward hook on one of
+them (or on every module), a forward of its own, an adapter in a projection's place -- runs the
+module's own forward for as long as that is so.
 """
 import types
+
+from torch.nn.modules import module as _nn
 
 from .. import kernels
 from .modules import Int8Rows, RW8Linear
@@ -28,6 +35,7 @@ def _covered(layer):
                 for n in ("q_proj", "k_proj", "v_proj", "o_proj")) and
             all(isinstance(getattr(m, n, None), RW8Linear)
                 for n in ("gate_proj", "up_proj", "down_proj")) and
+            "act_fn" in m._modules and
             all(getattr(n, "weight", None) is not None and hasattr(n, "variance_epsilon")
                 for n in norms))
 
@@ -60,9 +68,39 @@ def _norm(module, x, residual=None):
     return (codes, scale) if residual is None else (codes, scale, h)
 
 
+_ROWS = (("self_attn", "q_proj"), ("self_attn", "k_proj"), ("self_attn", "v_proj"),
+         ("mlp", "gate_proj"), ("mlp", "up_proj"), ("mlp", "down_proj"))
+
+
+def _watched(module):
+    d = module.__dict__
+    return d["_forward_pre_hooks"] or d["_forward_hooks"] or "forward" in d
+
+
+def _takes_rows(layer):
+    """Whether the modules that the 8-bit forward passes by, or hands 8-bit rows, are as
+    :func:`fuse_rw8_layers` found them and nothing watches their calls.  (Asked at every call, so in
+    plain dictionary lookups: 3 us a layer.)"""
+    if _nn._global_forward_pre_hooks or _nn._global_forward_hooks:
+        return False
+    mods = layer._modules
+    a, m = mods["self_attn"], mods["mlp"]
+    for parent, name in _ROWS:
+        p = mods[parent]._modules.get(name)
+        if not isinstance(p, RW8Linear) or _watched(p):
+            return False
+    return not (a._forward_pre_hooks or _watched(m) or _watched(m._modules["act_fn"]) or
+                _watched(mods["input_layernorm"]) or _watched(mods["post_attention_layernorm"]))
+
+
 def rw8_layer_forward(self, hidden_states, attention_mask=None, position_ids=None,
                       past_key_values=None, use_cache=False, position_embeddings=None, **kwargs):
     """A Llama decoder layer (transformers ``models/llama/modeling_llama.py``) on 8-bit rows."""
+    if not _takes_rows(self):
+        return type(self).forward(self, hidden_states, attention_mask=attention_mask,
+                                  position_ids=position_ids, past_key_values=past_key_values,
+                                  use_cache=use_cache, position_embeddings=position_embeddings,
+                                  **kwargs)
     dtype = hidden_states.dtype
     codes, scale = _norm(self.input_layernorm, hidden_states)
     attn, _ = self.self_attn(hidden_states=Int8Rows(codes, scale, dtype),
