@@ -41,9 +41,9 @@ def _covered(layer):
 
 
 def fuse_rw8_layers(model):
-    """Give every decoder layer of an RW8 Llama-architecture ``model`` the 8-bit forward above
-    (layers with other modules, and other models, are left as they are).  Returns how many layers
-    have it."""
+    """Give every decoder layer of an RW8 Llama-architecture ``model`` the 8-bit forward above.
+    Other models, and layers with other modules or with a forward of their own already (a dispatched
+    or offloaded model's), are left as they are.  Returns how many layers have it."""
     cfg = getattr(model, "config", None)
     if getattr(cfg, "model_type", None) != "llama" or \
             getattr(cfg, "hidden_act", None) not in ("silu", "swish"):
@@ -51,8 +51,11 @@ def fuse_rw8_layers(model):
     layers = getattr(getattr(model, "model", None), "layers", ())
     n = 0
     for layer in layers:
-        if _covered(layer):
+        own = layer.__dict__.get("forward")
+        if own is None and _covered(layer):
             layer.forward = types.MethodType(rw8_layer_forward, layer)
+            n += 1
+        elif getattr(own, "__func__", None) is rw8_layer_forward:
             n += 1
     return n
 

@@ -130,3 +130,27 @@ def test_forwards_and_adapters_put_in_after_fusing_are_called(model):
     mlp.up_proj = Adapter(mlp.up_proj)
     run(model)
     assert calls["norm"] == 2
+
+
+def test_layers_with_a_forward_of_their_own_keep_it(model):
+    """A wrapped layer is left as it is; one that is wrapped after it was fused stays wrapped."""
+    model, calls = model
+    first, second = model.model.layers
+    inner, seen = first.forward, []
+
+    def wrapped(*a, **k):
+        seen.append(1)
+        return inner(*a, **k)
+
+    first.forward = wrapped
+    assert fuse_rw8_layers(model) == 1 and first.forward is wrapped
+    run(model)
+    assert seen == [1] and calls["norm"] == 2
+    fused = second.forward
+    second.forward = lambda *a, **k: fused(*a, **k)
+    outer = second.forward
+    assert fuse_rw8_layers(model) == 0 and second.forward is outer
+    run(model)
+    assert seen == [1, 1] and calls["norm"] == 4
+    del first.forward, second.forward
+    assert fuse_rw8_layers(model) == 2 and fuse_rw8_layers(model) == 2
