@@ -285,6 +285,10 @@ class RocketModel:
     ``generate`` calls run :class:`~rocketllm_b200.speculative.SpeculativeDecoder` -- ``"on"``
     always, ``"auto"`` when the weights stream, ``"off"`` never; ``lookahead`` proposals per pass
     to start, adapted up to ``max_lookahead``.
+
+    ``rw8_layers``: give the layers of an RW8 (8-bit) Llama their forward on 8-bit rows
+    (:func:`~rocketllm_b200.quant.fuse_rw8_layers`); False keeps the model's own layer forward, in
+    which every projection quantizes its input itself.
     """
 
     def __init__(self, model_or_path, device="cuda", dtype=torch.bfloat16, vram_budget=None,
@@ -292,7 +296,7 @@ class RocketModel:
                  expert_streaming=True, kv_cache="auto", draft_model=None, speculative="auto",
                  lookahead=4, max_lookahead=8, expert_routing="host", expert_policy=None,
                  io_workers=4, host_budget=None, storage_depth=2, read_faults=None,
-                 **reference_knobs):
+                 rw8_layers=True, **reference_knobs):
         from .kv_cache import KV_CHOICES
         from .shards import INDEX
         from .speculative import SPEC_CHOICES
@@ -328,7 +332,8 @@ class RocketModel:
                 os.path.exists(os.path.join(str(model_or_path), INDEX)):
             self._init_from_shards(str(model_or_path), device, dtype, vram_budget, window,
                                    prefetching, copy_streams, chunk_bytes, io_workers,
-                                   host_budget, storage_depth, expert_streaming, read_faults)
+                                   host_budget, storage_depth, expert_streaming, read_faults,
+                                   rw8_layers)
             return
         if host_budget is not None:
             raise ValueError("host_budget applies to a layer-shard directory "
@@ -340,7 +345,8 @@ class RocketModel:
         else:
             model = model_or_path
         self.model = model.eval()
-        quant.fuse_rw8_layers(self.model)   # an RW8 Llama's layers; nothing for other models
+        if rw8_layers:
+            quant.fuse_rw8_layers(self.model)   # an RW8 Llama's layers; nothing for other models
         self.device = torch.device(device)
         layers = _decoder_layers(model)
         rest, layer_bytes = footprint(model)   # embeddings, final norm, lm_head: resident
@@ -399,7 +405,8 @@ class RocketModel:
 
     def _init_from_shards(self, root, device, dtype, vram_budget, window, prefetching,
                           copy_streams, chunk_bytes, io_workers=1, host_budget=None,
-                          storage_depth=2, expert_streaming=True, read_faults=None):
+                          storage_depth=2, expert_streaming=True, read_faults=None,
+                          rw8_layers=True):
         """Layer shards written by ``shards.split_rw4_layers``: the model is built on the meta
         device, the non-layer tensors come from ``rest.safetensors`` straight to the device, and
         each layer's blob is read from its file into pinned memory by positioned reads over
@@ -409,7 +416,7 @@ class RocketModel:
         self.device = torch.device(device)
         reader = LayerShardReader(root, io_workers=io_workers, faults=read_faults)
         self.shards = reader
-        model = build_skeleton(root, dtype).eval()
+        model = build_skeleton(root, dtype, rw8_layers).eval()
         self.model = model
         layers_path = reader.index["layers_path"]
         _materialize_rest(model, root, self.device, layers_path)

@@ -446,8 +446,9 @@ class LayerStager:
         self.reader.close()
 
 
-def build_skeleton(root, dtype=torch.bfloat16):
-    """The RW4 (or RW8) ``*ForCausalLM`` of ``root`` on the meta device (no storage allocated)."""
+def build_skeleton(root, dtype=torch.bfloat16, rw8_layers=True):
+    """The RW4 (or RW8) ``*ForCausalLM`` of ``root`` on the meta device (no storage allocated);
+    ``rw8_layers``: an RW8 Llama's layers with their 8-bit forward."""
     from transformers import AutoConfig, AutoModelForCausalLM
 
     from .quant import fuse_rw8_layers, quant_method_of
@@ -460,7 +461,8 @@ def build_skeleton(root, dtype=torch.bfloat16):
         model = AutoModelForCausalLM.from_config(config, dtype=dtype)
     if quant_method_of(q) == "rw8":
         convert_modules_rw8(model, skip)
-        fuse_rw8_layers(model)
+        if rw8_layers:
+            fuse_rw8_layers(model)
     else:
         convert_modules(model, skip)
     return model

@@ -154,3 +154,25 @@ def test_layers_with_a_forward_of_their_own_keep_it(model):
     assert seen == [1, 1] and calls["norm"] == 4
     del first.forward, second.forward
     assert fuse_rw8_layers(model) == 2 and fuse_rw8_layers(model) == 2
+
+
+def test_the_engine_leaves_layers_alone_when_asked(model, tmp_path):
+    import json
+
+    from rocketllm_b200.engine import RocketModel
+    from rocketllm_b200.quant.hf import RW8Config
+    from rocketllm_b200.shards import build_skeleton
+    model, calls = model
+    ids = torch.arange(12).view(2, 6)
+    with torch.no_grad():
+        want = run(model)
+        plain = RocketModel(model, device="cpu", dtype=torch.float32, rw8_layers=False)
+        assert torch.equal(plain(ids).logits, want) and calls["norm"] == 0
+        RocketModel(model, device="cpu", dtype=torch.float32)(ids)
+        assert calls["norm"] == 4
+    cfg = model.config.to_dict()
+    cfg["quantization_config"] = RW8Config().to_dict()
+    (tmp_path / "config.json").write_text(json.dumps(cfg))
+    for fused in (True, False):
+        layers = build_skeleton(str(tmp_path), rw8_layers=fused).model.layers
+        assert all(("forward" in layer.__dict__) == fused for layer in layers)
