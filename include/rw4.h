@@ -456,7 +456,8 @@ int rw4_ring_wait_compute(rw4_ring* ring, void* stream);
  * infinity as scale NaN, codes 0 (what reads it is NaN).  `dtype` (RW4_F32, RW4_BF16, RW4_F16) is
  * the type of every floating input; row strides are in elements, any value of at least 0 (rows
  * may overlap); codes, hidden and out are contiguous.  1 <= K <= 131056; M = 0 does nothing.  Any
- * length and alignment takes wide loads.
+ * length and alignment takes wide loads.  An output that overlaps another operand is refused, but
+ * for the forms in place that are named below.
  */
 
 /* codes, scale = quantized rows of x[M, K], or of silu(gate) * x when gate is not null
@@ -472,7 +473,8 @@ int rw4_int8_dequantize(const int8_t* codes, const float* scale, int64_t M, int6
 /* hidden = x + residual rounded to dtype (residual and hidden both null: hidden is x itself), and
  * codes, scale = quantized rows of hidden * rsqrt(mean(hidden^2) + eps) * weight, all in fp32 (for
  * any finite hidden, also where its squares or its products with the weight leave fp32).
- * hidden may be residual or x itself (same address, contiguous rows). */
+ * hidden may be residual or x itself (same address, contiguous rows), and overlaps neither
+ * otherwise. */
 int rw4_int8_rmsnorm(const void* x, int64_t x_stride, const void* residual,
                      int64_t residual_stride, const void* weight, int32_t dtype, int64_t M,
                      int64_t K, float eps, void* hidden, int8_t* codes, float* scale,

@@ -40,6 +40,21 @@ inline int launch_status(const char* what) { return cuda_status(cudaGetLastError
 
 inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
+// Whether the block of `bytes` at `block` shares a byte with M rows of `row_bytes`, `step` bytes apart.
+// (A null pointer is an operand that is not there.)
+inline bool meets(const void* block, int64_t bytes, const void* rows, int64_t row_bytes,
+                  int64_t M = 1, int64_t step = 0) {
+  if (!block || !rows) return false;
+  const uintptr_t b = reinterpret_cast<uintptr_t>(block);
+  uintptr_t r = reinterpret_cast<uintptr_t>(rows);
+  if (r + row_bytes <= b && M > 1 && step > 0) {   // on to the first row that ends after b
+    const uintptr_t i = (b - r - row_bytes) / step + 1;
+    if (i >= static_cast<uintptr_t>(M)) return false;
+    r += i * step;
+  }
+  return r < b + bytes && b < r + row_bytes;
+}
+
 inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s); }
 
 // Number of SMs of the current device, cached per device.

@@ -924,6 +924,11 @@ extern "C" int rw4_int8_linear(const int8_t* codes, const float* scale, int64_t 
   if (!aligned(scale, 4) || !aligned(weight_scale, 4) || !aligned(out, es) || !aligned(bias, es) ||
       !aligned(residual, es))
     return fail(RW4_EINVAL, "int8_linear: a pointer is not aligned to its type");
+  auto out_meets = [&](const void* p, int64_t bytes) { return meets(out, M * N * es, p, bytes); };
+  if (out_meets(codes, M * K) || out_meets(weight, N * K) || out_meets(scale, 4 * M) ||
+      out_meets(weight_scale, 4 * N) || out_meets(bias, N * es) ||
+      (residual != out && out_meets(residual, M * N * es)))
+    return fail(RW4_EINVAL, "int8_linear: out overlaps an input without being residual itself");
   Problem p;
   p.codes = codes;
   p.weight = weight;

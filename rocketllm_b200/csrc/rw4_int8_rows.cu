@@ -993,6 +993,30 @@ int run_rows_dtype(const RowArgs& a, int32_t dtype, cudaStream_t stream) {
 
 int elem_size(int32_t dtype) { return dtype == RW4_F32 ? 4 : 2; }
 
+// Whether the M x K codes or their scales at these addresses meet each other or rows of input (or the
+// new hidden rows): what another thread has yet to read could be written.
+bool outputs_meet(const RowArgs& a, int es) {
+  const int64_t codes = a.M * a.K, scale = 4 * a.M;
+  auto meet = [&](const void* p, int64_t ld) {
+    return rw4::meets(a.codes, codes, p, a.K * es, a.M, ld * es) ||
+           rw4::meets(a.scale, scale, p, a.K * es, a.M, ld * es);
+  };
+  return rw4::meets(a.codes, codes, a.scale, scale) || meet(a.x, a.x_ld) ||
+         meet(a.second, a.second_ld) || meet(a.hidden, a.K) ||
+         rw4::meets(a.codes, codes, a.weight, a.K * es) ||
+         rw4::meets(a.scale, scale, a.weight, a.K * es);
+}
+
+// Whether the hidden rows meet rows of input without being those very rows.
+bool hidden_meets(const RowArgs& a, int es) {
+  auto meet = [&](const void* p, int64_t ld) {
+    return !(p == a.hidden && ld == a.K) &&
+           rw4::meets(a.hidden, a.M * a.K * es, p, a.K * es, a.M, ld * es);
+  };
+  return meet(a.x, a.x_ld) || meet(a.second, a.second_ld) ||
+         rw4::meets(a.hidden, a.M * a.K * es, a.weight, a.K * es);
+}
+
 // The checks that every row entry point shares.
 int check_rows(const char* who, int32_t dtype, int64_t M, int64_t K) {
   if (dtype != RW4_F32 && dtype != RW4_BF16 && dtype != RW4_F16)
@@ -1103,6 +1127,8 @@ extern "C" int rw4_int8_quantize(const void* x, int64_t x_stride, const void* ga
   a.second_ld = M > 1 ? gate_stride : K;
   a.M = M;
   a.K = static_cast<int>(K);
+  if (outputs_meet(a, es))
+    return fail(RW4_EINVAL, "int8_quantize: codes or scale overlap an input or each other");
   cudaStream_t s = rw4::as_stream(stream);
   return gate ? run_rows_dtype<kGated>(a, dtype, s) : run_rows_dtype<kPlain>(a, dtype, s);
 }
@@ -1136,6 +1162,11 @@ extern "C" int rw4_int8_rmsnorm(const void* x, int64_t x_stride, const void* res
   a.M = M;
   a.K = static_cast<int>(K);
   a.eps = eps;
+  if (outputs_meet(a, es))
+    return fail(RW4_EINVAL, "int8_rmsnorm: codes or scale overlap another operand or each other");
+  if (hidden_meets(a, es))
+    return fail(RW4_EINVAL, "int8_rmsnorm: hidden overlaps an input without being x or residual "
+                "itself");
   cudaStream_t s = rw4::as_stream(stream);
   return residual ? run_rows_dtype<kNormRes>(a, dtype, s) : run_rows_dtype<kNorm>(a, dtype, s);
 }
@@ -1148,6 +1179,9 @@ extern "C" int rw4_int8_dequantize(const int8_t* codes, const float* scale, int6
   if (!codes || !scale || !out) return fail(RW4_EINVAL, "int8_dequantize: null pointer");
   if (!rw4::aligned(out, elem_size(out_dtype)) || !rw4::aligned(scale, 4))
     return fail(RW4_EINVAL, "int8_dequantize: a pointer is not aligned to its type");
+  const int64_t bytes = M * K * elem_size(out_dtype);
+  if (rw4::meets(out, bytes, codes, M * K) || rw4::meets(out, bytes, scale, 4 * M))
+    return fail(RW4_EINVAL, "int8_dequantize: out overlaps an input");
   cudaStream_t s = rw4::as_stream(stream);
   if (out_dtype == RW4_F32)
     return launch_dequant(codes, scale, M, K, static_cast<float*>(out), s);

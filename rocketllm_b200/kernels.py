@@ -298,7 +298,8 @@ def int8_rmsnorm(x, weight, eps, residual=None, out=None, hidden=None):
 
     The normed row is not rounded before it is quantized (fp32, as :func:`int8_quantize`).
     ``weight [K]`` has x's type.  ``hidden``: the tensor to write ``h`` to (contiguous; it may be
-    ``x`` or ``residual`` itself).
+    ``x`` or ``residual`` itself; any other overlap of an output with another operand is refused,
+    here and in the other 8-bit calls).
     """
     if _native is not None and out is None and hidden is None:
         done = _native.int8_rmsnorm(x, weight, eps, residual)

@@ -137,3 +137,45 @@ def test_scales_whose_product_is_small(cuda, m, k, n, path, dtype):
     if m > 1:
         check(y[:m - 1], q[:m - 1], ss[:m - 1], tt)
         assert not y[m // 2].any() and not y[:m - 1, n // 2].any()
+
+
+def test_outputs_beside_their_operands_are_taken(cuda):
+    """Operands side by side in one buffer, outputs between strided rows, and in place: none of them
+    overlaps.  Outputs that do are refused through the Python calls, too."""
+    m, k = 5, 128
+    buf = torch.zeros(1 << 16, dtype=BF, device="cuda")
+    x = buf[:m * k].view(m, k)
+    x.copy_(randn(1, m, k))
+    want = kernels.int8_quantize(x.clone())
+    after = buf[m * k:].view(torch.int8)
+    codes = after[:m * k].view(m, k)
+    scale = after[m * k:m * k + 4 * m].view(F32)
+    assert all(torch.equal(a, b) for a, b in zip(kernels.int8_quantize(x, out=(codes, scale)), want))
+    # rows far apart, the outputs in the gap between the first two
+    apart = buf.as_strided((m, k), (4096, 1), 8192)
+    apart.copy_(x)
+    gap = buf[8192 + k:8192 + 4096].view(torch.int8)
+    out = (gap[:m * k].view(m, k), gap[m * k:m * k + 4 * m].view(F32))
+    assert all(torch.equal(a, b) for a, b in zip(kernels.int8_quantize(apart, out=out), want))
+    w, r = randn(2, k), randn(3, m, k)
+    want = kernels.int8_rmsnorm(x.clone(), w, 1e-5, residual=r)
+    xx = x.clone()
+    assert all(torch.equal(a, b) for a, b in
+               zip(kernels.int8_rmsnorm(xx, w, 1e-5, residual=r, hidden=xx), want))
+    both = x.clone()      # x, residual and hidden in one
+    want = kernels.int8_rmsnorm(x.clone(), w, 1e-5, residual=x.clone())
+    assert all(torch.equal(a, b) for a, b in
+               zip(kernels.int8_rmsnorm(both, w, 1e-5, residual=both, hidden=both), want))
+    flat = torch.zeros(m * k + 1, dtype=BF, device="cuda")
+    for call in (lambda: kernels.int8_rmsnorm(flat[1:].view(m, k), w, 1e-5, residual=r,
+                                              hidden=flat[:-1].view(m, k)),
+                 lambda: kernels.int8_rmsnorm(flat[:k].expand(m, k), w, 1e-5, residual=r,
+                                              hidden=flat[:-1].view(m, k)),
+                 lambda: kernels.int8_quantize(x, out=(x.view(torch.int8).flatten()[:m * k].view(m, k),
+                                                  scale))):
+        with pytest.raises(RuntimeError, match="overlap"):
+            call()
+    q, s, wq, ws, _, res = operands(4, m, k, 96, residual=True)
+    flat = torch.zeros(m * 96 + 1, dtype=BF, device="cuda")
+    with pytest.raises(RuntimeError, match="overlap"):
+        kernels.int8_linear(q, s, wq, ws, residual=flat[1:].view(m, 96), out=flat[:-1].view(m, 96))
