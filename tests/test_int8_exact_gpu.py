@@ -179,3 +179,48 @@ def test_outputs_beside_their_operands_are_taken(cuda):
     flat = torch.zeros(m * 96 + 1, dtype=BF, device="cuda")
     with pytest.raises(RuntimeError, match="overlap"):
         kernels.int8_linear(q, s, wq, ws, residual=flat[1:].view(m, 96), out=flat[:-1].view(m, 96))
+
+
+@pytest.mark.parametrize("path,m", [(1, 4), (1, 100), (2, 64), (2, 600)])
+def test_products_read_what_the_launches_before_them_wrote(cuda, path, m):
+    """Weights and activations quantized into the same buffers again and again, their codes other
+    ones each time, and multiplied at once: launches overlap their prologues, and each product
+    gives what it gives alone."""
+    n, k = 2048, 4096
+    weights = [randn(s, n, k) for s in range(4)]
+    xs = [randn(10 + s, m, k) for s in range(3)]
+    w = (torch.empty(n, k, dtype=torch.int8, device="cuda"), torch.empty(n, device="cuda"))
+    q = (torch.empty(m, k, dtype=torch.int8, device="cuda"), torch.empty(m, device="cuda"))
+    res = randn(20, m, n)
+
+    def product(i, out=None):
+        kernels.int8_quantize(xs[i % 3], out=q)
+        kernels.int8_quantize(weights[i % 4], out=w)
+        return kernels.int8_linear(*q, *w, residual=res, path=path, out=out)
+
+    want = []
+    for i in range(12):
+        want.append(product(i).clone())
+        torch.cuda.synchronize()
+    assert not any(torch.equal(want[i], want[j]) for i in range(12) for j in range(i))
+    got = [torch.empty_like(res) for _ in range(48)]
+    for i in range(48):        # the weights last
+        product(i, got[i])
+    for i in range(48):
+        assert torch.equal(got[i], want[i % 12])
+    for i in range(48):        # the activations last
+        kernels.int8_quantize(weights[i % 4], out=w)
+        kernels.int8_quantize(xs[i % 3], out=q)
+        kernels.int8_linear(*q, *w, residual=res, path=path, out=got[i])
+    for i in range(48):
+        assert torch.equal(got[i], want[i % 12])
+    # in a graph, whose launches follow one another without the host
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for i in range(48):
+            product(i, got[i])
+    for g in got:
+        g.zero_()
+    graph.replay()
+    for i in range(48):
+        assert torch.equal(got[i], want[i % 12])
