@@ -455,9 +455,11 @@ int rw4_ring_wait_compute(rw4_ring* ring, void* stream);
  * fp32.  A row with a < 2^-119 is stored as scale 0, codes 0; a row that holds a NaN or an
  * infinity as scale NaN, codes 0 (what reads it is NaN).  `dtype` (RW4_F32, RW4_BF16, RW4_F16) is
  * the type of every floating input; row strides are in elements, any value of at least 0 (rows
- * may overlap); codes, hidden and out are contiguous.  1 <= K <= 131056; M = 0 does nothing.  Any
- * length and alignment takes wide loads.  An output that overlaps another operand is refused, but
- * for the forms in place that are named below.
+ * may overlap); codes, hidden and out are contiguous.  1 <= K <= 131056; M = 0 does nothing.  The
+ * quantizer and the norm read rows of any length and alignment in wide loads.  Hidden rows are
+ * written in wide stores where hidden starts on 16 bytes and codes on 8, and rw4_int8_dequantize
+ * reads and writes wide where codes and out start on 16; elsewhere these go value by value.  An
+ * output that overlaps another operand is refused, but for the forms in place named below.
  */
 
 /* codes, scale = quantized rows of x[M, K], or of silu(gate) * x when gate is not null
