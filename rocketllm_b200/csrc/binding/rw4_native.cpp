@@ -261,4 +261,12 @@ PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_rw4_native",
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__rw4_native() { return PyModule_Create(&kModule); }
+// `torch_version`: what this was compiled against; kernels.py takes it beside that torch alone.
+PyMODINIT_FUNC PyInit__rw4_native() {
+  PyObject* m = PyModule_Create(&kModule);
+  if (m && PyModule_AddStringConstant(m, "torch_version", RW4_TORCH_VERSION) < 0) {
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}

@@ -13,6 +13,14 @@ from . import _lib
 
 try:   # host fast path of the 8-bit operators; without it the same calls are made through ctypes
     from . import _rw4_native as _native
+    if getattr(_native, "torch_version", None) != torch.__version__:
+        # compiled against another torch's tensors: what they look like inside may have changed
+        import warnings
+        warnings.warn("rocketllm_b200/_rw4_native.so was built against torch "
+                      f"{getattr(_native, 'torch_version', '(unknown)')}, this is "
+                      f"{torch.__version__}: it is not used (rebuild with rocketllm_b200/csrc/"
+                      "build.py)")
+        _native = None
 except ImportError:
     _native = None
 
