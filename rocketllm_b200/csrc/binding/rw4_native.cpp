@@ -40,7 +40,8 @@ int dtype_code(at::ScalarType t) {
   return -1;
 }
 
-// t [..., K] as rows with one stride between them, without a copy.
+// t [..., K] as rows with one stride between them, without a copy (the halves of a [B, S, 2 K]
+// projection are such rows).
 bool as_rows(const at::Tensor& t, int64_t& m, int64_t& k, int64_t& ld) {
   const int64_t d = t.dim();
   if (d < 1) return false;
@@ -51,9 +52,14 @@ bool as_rows(const at::Tensor& t, int64_t& m, int64_t& k, int64_t& ld) {
     ld = t.stride(0);
     return true;
   }
-  if (!t.is_contiguous()) return false;
-  m = t.numel() / k;
+  m = 1;
   ld = k;
+  for (int64_t i = d - 2; i >= 0; --i) {   // outwards; m rows so far, ld apart
+    const int64_t n = t.size(i);
+    if (n != 1 && m == 1) ld = t.stride(i);
+    else if (n > 1 && m > 1 && t.stride(i) != m * ld) return false;
+    m *= n;
+  }
   return true;
 }
 

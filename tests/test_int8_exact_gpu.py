@@ -224,3 +224,27 @@ def test_products_read_what_the_launches_before_them_wrote(cuda, path, m):
     graph.replay()
     for i in range(48):
         assert torch.equal(got[i], want[i % 12])
+
+
+def test_native_path_takes_rows_of_any_dimension(cuda):
+    """Views of three and four dimensions with one stride between their rows are not declined, others
+    are, and both give what compact copies give."""
+    gu = randn(1, 2, 3, 4, 512)
+    w = randn(2, 256)
+    one = [gu[..., :256], gu[..., 256:], gu[:1, :, :, :256], gu[:, :, :, 8:264], gu[:, :1, :1, :256],
+           gu[:1, :1, :1, 5:261], gu[:1, :1, ::2, :256], gu[:0, :, :, :256], gu[:, :0, :, :256],
+           gu[:1, :1, :1, :256].expand(2, 3, 4, 256)]
+    many = [gu[:, :, ::3, :256], gu[:, :2, :, :256], gu.transpose(0, 1)[..., :256],
+            gu[:, :, :1, :256].expand(2, 3, 4, 256)]
+    for i, v in enumerate(one + many):
+        c = v.clone(memory_format=torch.contiguous_format)
+        calls = [(kernels._native.int8_quantize, (v, v), kernels.int8_quantize, (c, c)),
+                 (kernels._native.int8_rmsnorm, (v, w, 1e-5, v), kernels.int8_rmsnorm,
+                  (c, w, 1e-5, c))]
+        for native, args, plain, copies in calls:
+            got = native(*args)
+            assert (got is not None) == (i < len(one))
+            want = plain(*copies)
+            for g in (got, plain(*args)):
+                if g is not None:
+                    assert all(a.shape == b.shape and torch.equal(a, b) for a, b in zip(g, want))
