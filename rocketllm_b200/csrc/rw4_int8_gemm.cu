@@ -383,7 +383,9 @@ __global__ void __launch_bounds__(SplitCfg<BN>::kThreads)
       bulk_send(map_rank(sb + C::kOffPart + rank * run * kColBytes, et), sb + et * run * kColBytes,
                 share(et) * kColBytes, map_rank(parts, et));
   }
-  if (epi && ok && share(rank) > 0 && (splits == 1 || mbar_wait(parts, 0, status))) {
+  // (A CTA whose own sums are not there waits for the others' all the same, as long as a wait lasts:
+  // they may be on their way, and must not find its shared memory, or their senders', gone.)
+  if (epi && share(rank) > 0 && (splits == 1 || mbar_wait(parts, 0, status)) && ok) {
     const uint32_t got = sb + (splits > 1 ? C::kOffPart : 0);
     const T* res = static_cast<const T*>(e.residual);
     T* out = static_cast<T*>(e.out);
