@@ -784,13 +784,14 @@ int set_smem(const void* kern, int bytes, std::atomic<uint64_t>& done) {
   return RW4_OK;
 }
 
-int maps(const Problem& p, int box_tokens, CUtensorMap* w, CUtensorMap* x) {
-  int st = make_tensor_map_2d(w, p.weight, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.N, p.K, p.K, BMW,
-                              BK, CU_TENSOR_MAP_SWIZZLE_128B);
-  if (st == RW4_OK)
-    st = make_tensor_map_2d(x, p.codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.M, p.K, p.K,
-                            box_tokens, BK, CU_TENSOR_MAP_SWIZZLE_128B);
-  return st;
+int weight_map(const Problem& p, CUtensorMap* w) {
+  return make_tensor_map_2d(w, p.weight, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.N, p.K, p.K, BMW, BK,
+                            CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+int token_map(const Problem& p, int box_tokens, CUtensorMap* x) {
+  return make_tensor_map_2d(x, p.codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.M, p.K, p.K, box_tokens,
+                            BK, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 int launch(const void* kern, int grid, int threads, int smem, int cluster, cudaStream_t stream,
@@ -821,7 +822,8 @@ int launch_split(const Problem& p) {
   static std::atomic<uint64_t> done{0};
   int st = set_smem(kern, C::kSmem, done);
   CUtensorMap w, x;
-  if (st == RW4_OK) st = maps(p, BN, &w, &x);
+  if (st == RW4_OK) st = weight_map(p, &w);
+  if (st == RW4_OK) st = token_map(p, BN, &x);
   if (st != RW4_OK) return st;
   int M = (int)p.M, N = (int)p.N, nkb = (int)((p.K + BK - 1) / BK);
   int m_tiles = (M + BN - 1) / BN;
@@ -861,8 +863,10 @@ int launch_pair(const Problem& p) {
   for (g.cut = 0; rest && g.cut < 2 && (rest << (g.cut + 1)) <= pairs;) ++g.cut;
   g.items = g.full + (rest << g.cut);
   CUtensorMap w, x, strip;
-  if (st == RW4_OK) st = maps(p, kPairTokens / 2, &w, &x);
-  if (st == RW4_OK) st = maps(p, (kPairTokens >> g.cut) / 2, &w, &strip);
+  if (st == RW4_OK) st = weight_map(p, &w);
+  if (st == RW4_OK) st = token_map(p, kPairTokens / 2, &x);
+  if (st == RW4_OK && g.cut) st = token_map(p, (kPairTokens >> g.cut) / 2, &strip);
+  if (!g.cut) strip = x;
   if (st != RW4_OK) return st;
   Epilogue e = p.e;
   unsigned int* status = p.status;
