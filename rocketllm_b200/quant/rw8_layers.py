@@ -17,27 +17,36 @@ slots) takes the same path.
 
 The norms and the MLP are not called as modules here, and the projections that read 8-bit rows get
 :class:`Int8Rows`.  So a layer in which something waits for those calls -- a forward hook on one of
-them (or on every module), a forward of its own, an adapter in a projection's place -- runs the
-module's own forward for as long as that is so.
+them (or on every module), a forward of its own, another module in its place -- runs the module's own
+forward for as long as that is so.
 """
 import types
 
+from torch import nn
 from torch.nn.modules import module as _nn
 
 from .. import kernels
 from .modules import Int8Rows, RW8Linear
 
 
+def _passed_by(layer):
+    """The types of the modules whose calls the 8-bit forward replaces."""
+    mods = layer._modules
+    m = mods.get("mlp")
+    return [type(mods.get("input_layernorm")), type(mods.get("post_attention_layernorm")), type(m),
+            type(m._modules.get("act_fn") if m is not None else None)]
+
+
 def _covered(layer):
+    from transformers.activations import ACT2FN
+    from transformers.models.llama.modeling_llama import LlamaMLP, LlamaRMSNorm
     a, m = getattr(layer, "self_attn", None), getattr(layer, "mlp", None)
-    norms = [getattr(layer, n, None) for n in ("input_layernorm", "post_attention_layernorm")]
     return (all(isinstance(getattr(a, n, None), RW8Linear)
                 for n in ("q_proj", "k_proj", "v_proj", "o_proj")) and
             all(isinstance(getattr(m, n, None), RW8Linear)
                 for n in ("gate_proj", "up_proj", "down_proj")) and
-            "act_fn" in m._modules and
-            all(getattr(n, "weight", None) is not None and hasattr(n, "variance_epsilon")
-                for n in norms))
+            _passed_by(layer)[:3] == [LlamaRMSNorm, LlamaRMSNorm, LlamaMLP] and
+            type(m.act_fn) in (nn.SiLU, type(ACT2FN["silu"])))
 
 
 def fuse_rw8_layers(model):
@@ -53,6 +62,7 @@ def fuse_rw8_layers(model):
     for layer in layers:
         own = layer.__dict__.get("forward")
         if own is None and _covered(layer):
+            layer._rw8_passed_by = _passed_by(layer)
             layer.forward = types.MethodType(rw8_layer_forward, layer)
             n += 1
         elif getattr(own, "__func__", None) is rw8_layer_forward:
@@ -84,7 +94,8 @@ def _takes_rows(layer):
     """Whether the modules that the 8-bit forward passes by, or hands 8-bit rows, are as
     :func:`fuse_rw8_layers` found them and nothing watches their calls.  (Asked at every call, so in
     plain dictionary lookups: 3 us a layer.)"""
-    if _nn._global_forward_pre_hooks or _nn._global_forward_hooks:
+    if _nn._global_forward_pre_hooks or _nn._global_forward_hooks or \
+            _passed_by(layer) != layer._rw8_passed_by:
         return False
     mods = layer._modules
     a, m = mods["self_attn"], mods["mlp"]

@@ -132,6 +132,30 @@ def test_forwards_and_adapters_put_in_after_fusing_are_called(model):
     assert calls["norm"] == 2
 
 
+def test_other_modules_in_the_place_of_those_passed_by_are_called(model):
+    """Another activation or norm, put in before or after the layers were fused."""
+    model, calls = model
+    first, second = model.model.layers
+
+    class Doubled(type(first.input_layernorm)):
+        def forward(self, x):
+            return 2 * super().forward(x)
+
+    first.mlp.act_fn = torch.nn.GELU()
+    assert fuse_rw8_layers(model) == 1
+    second.mlp.act_fn = torch.nn.GELU()
+    got = run(model)
+    assert calls == {"norm": 0, "gated": 0}
+    second.__dict__.pop("forward")
+    assert torch.equal(run(model), got)        # the modules' own
+    first.mlp.act_fn, second.mlp.act_fn = torch.nn.SiLU(), torch.nn.SiLU()
+    first.input_layernorm.__class__ = Doubled
+    assert fuse_rw8_layers(model) == 1         # not the first
+    second.post_attention_layernorm.__class__ = Doubled
+    run(model)
+    assert calls == {"norm": 0, "gated": 0}
+
+
 def test_layers_with_a_forward_of_their_own_keep_it(model):
     """A wrapped layer is left as it is; one that is wrapped after it was fused stays wrapped."""
     model, calls = model
