@@ -860,8 +860,8 @@ struct RingShape {
 };
 
 // How a ring takes rows of nvec vectors; false where it does not: short rows (a warp each), or
-// fewer than two rows for every CTA (then a CTA per row is faster: 1001 x 5632, norm 6.1 us against
-// 7.9).  pad: bytes around a piece in shared memory (0: whole rows, as they are).
+// fewer than two rows for every CTA (then a CTA per row is faster: 1001 x 5632, norm 5.6 us against
+// 7.3).  pad: bytes around a piece in shared memory (0: whole rows, as they are).
 template <typename T, int MODE>
 bool ring_shape(const RowArgs& a, int nvec, int pad, RingShape& r) {
   if (nvec <= 128) return false;
@@ -878,8 +878,8 @@ bool ring_shape(const RowArgs& a, int nvec, int pad, RingShape& r) {
     auto fits = [&](int n) { return 227 * 1024 / (fixed + n * stage + 2048); };
     // two stages as long as two CTAs an SM hold them (or the one that its threads allow): below
     // that a second CTA hides more than a second stage (swiglu 2048 x 14336: 31.5 us with two CTAs
-    // of one stage, 34.0 with one of two; norm with residual 8192 x 8192: 73 us with two CTAs of two
-    // stages, 83 with four of one)
+    // of one stage, 34.0 with one of two; norm with residual 8192 x 8192: 77 us with two CTAs of two
+    // stages, 79 with four of one)
     r.stages = fits(2) >= (per_sm < 2 ? per_sm : 2) ? 2 : 1;
     const int f = fits(r.stages);
     if (f < 1) continue;

@@ -7,7 +7,8 @@ of ``rocketllm/quant/registry.py:33``):
     X.weight         int8  [N, K]
     X.weight_scale   fp32  [N, 1]     value = code * scale
 
-the layout of a channel-wise ``int-quantized`` compressed-tensors checkpoint, which the reference
+the tensors of a channel-wise ``int-quantized`` compressed-tensors checkpoint (whose config still has
+to say ``quant_method: "rw8"``: nothing else selects this backend), which the reference
 expands to a bf16 scratch copy on every fetch (``rocketllm/quant/safetensors_quant.py:244-293``).
 Here ``needs_scratch`` is False: the library multiplies the codes as they are.
 """
